@@ -10,6 +10,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 from setuptools import setup
@@ -37,13 +38,17 @@ class HipBuildExt(build_ext):
         out = Path(self.get_ext_fullpath(ext.name))
         out.parent.mkdir(parents=True, exist_ok=True)
         hipcc = os.environ.get("HIPCC", "hipcc")
-        cmd = [
+        compile_cmd = [
             hipcc,
             f"--offload-arch={ARCH}",
             "-O3",
             "-std=c++17",
             "-fPIC",
-            "-shared",
+            # some forms of the packed fp32 instructions have given wrong results on gfx950
+            "-Xclang",
+            "-target-feature",
+            "-Xclang",
+            "-packed-fp32-ops",
             "-DTORCH_EXTENSION_NAME=_C",
             "-DUSE_ROCM",
             "-DTORCH_API_INCLUDE_EXTENSION_H",
@@ -51,9 +56,20 @@ class HipBuildExt(build_ext):
             f"-I{pybind11.get_include()}",
             f"-I{sysconfig.get_paths()['include']}",
         ]
-        cmd += [f"-I{inc}" for inc in includes]
-        cmd += sources
-        cmd += ["-o", str(out)]
+        compile_cmd += [f"-I{inc}" for inc in includes]
+        objects_dir = Path(self.build_temp)
+        objects_dir.mkdir(parents=True, exist_ok=True)
+        objects = [str(objects_dir / (Path(src).stem + ".o")) for src in sources]
+
+        def compile_one(src, obj):
+            cmd = [*compile_cmd, "-c", src, "-o", obj]
+            print(" ".join(cmd), flush=True)
+            subprocess.check_call(cmd)
+
+        with ThreadPoolExecutor(max_workers=int(os.environ.get("MAX_JOBS", 8))) as pool:
+            for job in [pool.submit(compile_one, *pair) for pair in zip(sources, objects)]:
+                job.result()
+        cmd = [hipcc, f"--offload-arch={ARCH}", "-fPIC", "-shared", *objects, "-o", str(out)]
         cmd += [f"-L{d}" for d in libdirs]
         cmd += ["-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-ltorch_hip", "-lamdhip64"]
         print(" ".join(cmd), flush=True)
