@@ -47,6 +47,21 @@ def has_extension() -> bool:
 
 from .grad_scaler import GradScaler  # noqa: E402
 from .clip_grad import clip_grad_norm_, get_grad_norm  # noqa: E402
+from .kv_cache import KVCache, cache_attention  # noqa: E402
 from .optim import FusedAdamW  # noqa: E402
+from .rope import rope_tables, rotary_embedding  # noqa: E402
+from .speculative import DraftVerdict, verify_draft  # noqa: E402
 
-__all__ = ["GradScaler", "FusedAdamW", "clip_grad_norm_", "get_grad_norm", "has_extension"]
+__all__ = [
+    "GradScaler",
+    "FusedAdamW",
+    "KVCache",
+    "DraftVerdict",
+    "cache_attention",
+    "clip_grad_norm_",
+    "get_grad_norm",
+    "has_extension",
+    "rope_tables",
+    "rotary_embedding",
+    "verify_draft",
+]

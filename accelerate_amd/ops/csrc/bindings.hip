@@ -648,7 +648,10 @@ std::vector<at::Tensor> dropout_add_ln_bwd(at::Tensor dy, at::Tensor s, at::Tens
   return {dx, dz, folded.narrow(0, 0, d), folded.narrow(0, d, d)};
 }
 
+void bind_serving(pybind11::module_& m);  // serving_bindings.hip
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_serving(m);
   m.def("layernorm_fwd", &layernorm_fwd, "fused bf16 LayerNorm forward");
   m.def("layernorm_bwd", &layernorm_bwd, "fused bf16 LayerNorm backward");
   m.def("dropout_add_ln_fwd", &dropout_add_ln_fwd,

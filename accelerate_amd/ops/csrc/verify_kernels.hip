@@ -1,0 +1,322 @@
+// Verification of drafted tokens against the target's probabilities, from
+// given random numbers.
+//
+// Node 0 is the last token that stands; a drafted node i > 0 follows its
+// parent, and target row i is the target's distribution after node i. From
+// the root on, with w the weights of the current node's row:
+//   sampled drafts (a chain, with the distribution q that each was drawn
+//     from): take token x of the child iff u_i q(x) < p(x); at the first
+//     refusal the answer comes from max(p - q, 0).
+//   certain drafts (a chain or a tree): the children in order; take child i
+//     iff u_i r < p(x), where r = 1 - the mass of the siblings refused before
+//     it; where none is taken the answer comes from p without those.
+// The answer is the first token whose cumulative weight exceeds u_0 times the
+// sum of all. So the tokens that come out are distributed as the target's.
+//
+// All comparisons and sums are in 64 bits: they decide whole numbers, and the
+// sum over a vocabulary of 10^5 in 32 bits would move the borders between
+// tokens by about their own width.
+//
+// Bound by latency and then by reading one row (with q two) a sequence. The
+// walk needs one value (two) a node, read by a thread each, and is done by
+// every workgroup for itself, so that a grid over chunks of the vocabulary
+// can sum its row at once, without a launch between; a second kernel finds
+// the chunk and the token in it.
+
+#include "serving.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 2048;     // vocabulary entries a workgroup sums
+constexpr int kMaxNodes = 1024;  // of a tree, root included
+
+template <typename T>
+__device__ __forceinline__ double wide(T x) { return (double)(float)x; }
+
+__device__ __forceinline__ double uniform_at(const VerifyArgs& a, int b, int i) {
+  return a.uniform_is_64 ? reinterpret_cast<const double*>(a.uniforms)[b * a.ub + i]
+                         : (double)reinterpret_cast<const float*>(a.uniforms)[b * a.ub + i];
+}
+
+// What the answer is drawn from: 0 the row as it is, 1 less the draft's, 2 without tokens
+enum Residual { kRow = 0, kLess = 1, kWithout = 2 };
+
+// meta of a sequence: last node, residual, tokens left out, those tokens
+constexpr int kMetaHead = 3;
+
+template <typename T>
+__device__ __forceinline__ double weight_at(const T* p, const T* q, int residual, int64_t x) {
+  double w = wide(p[x]);
+  if (residual == kLess) w -= wide(q[x]);
+  return w > 0. ? w : 0.;  // NaN too
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
+  __shared__ double p_of[kMaxNodes], q_of[kMaxNodes];
+  __shared__ int token_of[kMaxNodes], parent_of[kMaxNodes], without[kMaxNodes];
+  __shared__ int path[kMaxNodes];
+  __shared__ int s_last, s_residual, s_without, s_count, s_first;
+  __shared__ double sums[kThreads / 64];
+  const int b = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
+  const T* target = reinterpret_cast<const T*>(a.target) + b * a.tb;
+  const T* draft = a.draft ? reinterpret_cast<const T*>(a.draft) + b * a.db : nullptr;
+
+  if (tid == 0) s_first = a.T;
+  for (int i = tid; i < a.T; i += kThreads) {
+    const int64_t token = a.tokens[b * a.kb + i];
+    const int64_t parent = i == 0 ? -1 : (a.parents ? a.parents[b * a.pb + i] : (int64_t)i - 1);
+    // a node without a token of the vocabulary, or that follows none before it, is none
+    const bool is = i > 0 && token >= 0 && token < a.V && parent >= 0 && parent < i;
+    token_of[i] = is ? (int)token : -1;
+    parent_of[i] = is ? (int)parent : -1;
+    p_of[i] = is ? wide(target[parent * a.tt + token]) : 0.;
+    q_of[i] = is && draft ? wide(draft[parent * a.dt + token]) : 0.;
+  }
+  __syncthreads();
+
+  if (!a.parents) {  // a chain ends at the first node that is none or not taken
+    for (int i = 1 + tid; i < a.T; i += kThreads) {
+      const double u = uniform_at(a, b, i);
+      const bool taken = token_of[i] >= 0 && (draft ? u * q_of[i] < p_of[i] : u < p_of[i]);
+      if (!taken) atomicMin(&s_first, i);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      const int last = s_first - 1;
+      const bool refused = s_first < a.T && token_of[s_first] >= 0;
+      s_last = last;
+      s_count = last;
+      s_residual = !refused ? kRow : draft ? kLess : kWithout;
+      s_without = refused && !draft ? 1 : 0;
+      if (s_without) without[0] = token_of[s_first];
+    }
+    for (int i = tid; i < s_first; i += kThreads) path[i] = i;
+  } else if (tid == 0) {
+    // children come after their parents, so one pass in order is the walk
+    int cur = 0, n = 0, count = 0;
+    double left = 1.;
+    path[0] = 0;
+    for (int i = 1; i < a.T; ++i) {
+      if (parent_of[i] != cur) continue;
+      bool again = false;  // a token refused before has nothing left
+      for (int j = 0; j < n; ++j) again |= without[j] == token_of[i];
+      if (again) continue;
+      if (uniform_at(a, b, i) * left < p_of[i]) {
+        cur = i;
+        n = 0;
+        left = 1.;
+        path[++count] = i;
+      } else {
+        left -= p_of[i];
+        without[n++] = token_of[i];
+      }
+    }
+    s_last = cur;
+    s_count = count;
+    s_residual = n ? kWithout : kRow;
+    s_without = n;
+  }
+  __syncthreads();
+
+  const int last = s_last, residual = s_residual, n_without = s_without;
+  if (chunk == 0) {
+    int* meta = a.meta + (int64_t)b * (kMetaHead + a.T);
+    if (tid == 0) {
+      meta[0] = last;
+      meta[1] = residual;
+      meta[2] = n_without;
+      a.counts[b] = s_count;
+    }
+    for (int i = tid; i < n_without; i += kThreads) meta[kMetaHead + i] = without[i];
+    for (int i = tid; i < a.T; i += kThreads) {
+      a.path[(int64_t)b * a.T + i] = i <= s_count ? path[i] : -1;
+      if (i != s_count) a.out_tokens[(int64_t)b * a.T + i] = i < s_count ? token_of[path[i + 1]] : -1;
+    }
+  }
+
+  const T* p = target + last * a.tt;
+  const T* q = residual == kLess ? draft + last * a.dt : nullptr;
+  const int64_t from = (int64_t)chunk * kChunk, to = min(from + kChunk, a.V);
+  double sum = 0.;
+  for (int64_t x = from + tid; x < to; x += kThreads) {
+    double w = weight_at(p, q, residual, x);
+    for (int j = 0; j < n_without; ++j)
+      if (without[j] == x) w = 0.;
+    sum += w;
+  }
+#pragma unroll
+  for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
+  if ((tid & 63) == 0) sums[tid >> 6] = sum;
+  __syncthreads();
+  if (tid == 0) a.partial[(int64_t)b * a.chunks + chunk] = sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+// The sums of a value over the threads up to each one, into ends[1..kThreads];
+// ends[0] = 0. Sums that are joined in another order may fall by a rounding
+// where a value is tiny, so a border is looked for as the first that passes it.
+__device__ __forceinline__ void scan(double x, double* ends, double* shared) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const double y = __shfl_up(x, m);
+    if (lane >= m) x += y;
+  }
+  if (lane == 63) shared[wave] = x;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) x += shared[w];
+  ends[tid + 1] = x;
+  if (tid == 0) ends[0] = 0.;
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) verify_answer_kernel(VerifyArgs a) {
+  __shared__ double weights[kChunk];
+  __shared__ double ends[kThreads + 1], shared[kThreads / 64];
+  __shared__ double s_base;
+  __shared__ int s_thread, s_chunk, s_positive;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int* meta = a.meta + (int64_t)b * (kMetaHead + a.T);
+  const int last = meta[0], residual = meta[1], n_without = meta[2];
+  const T* p = reinterpret_cast<const T*>(a.target) + b * a.tb + last * a.tt;
+  const T* q = residual == kLess ? reinterpret_cast<const T*>(a.draft) + b * a.db + last * a.dt : nullptr;
+  int64_t* out = a.out_tokens + (int64_t)b * a.T + a.counts[b];
+  const double u = fmax(uniform_at(a, b, 0), 0.);
+  const double* partial = a.partial + (int64_t)b * a.chunks;
+  if (tid == 0) {
+    s_thread = kThreads;
+    s_positive = -1;
+  }
+
+  // the chunk: each thread has a run of them
+  const int per = (a.chunks + kThreads - 1) / kThreads;
+  const int c0 = min(tid * per, a.chunks), c1 = min(c0 + per, a.chunks);
+  double sum = 0.;
+  int positive = -1;
+  for (int i = c0; i < c1; ++i) {
+    sum += partial[i];
+    if (partial[i] > 0.) positive = i;
+  }
+  scan(sum, ends, shared);
+  if (positive >= 0) atomicMax(&s_positive, positive);
+  double threshold = u * ends[kThreads];
+  if (ends[tid + 1] > threshold && positive >= 0) atomicMin(&s_thread, tid);
+  __syncthreads();
+
+  if (s_positive < 0) {
+    // No weight at all. A residual that has none (a draft that covered all of
+    // the target) gives way to the row itself; that, to token 0. Rare: the
+    // whole workgroup goes over the row, twice.
+    double row = 0.;
+    if (residual != kRow)
+      for (int64_t x = tid; x < a.V; x += kThreads) row += weight_at(p, q, kRow, x);
+    __syncthreads();
+    scan(row, ends, shared);
+    threshold = u * ends[kThreads];
+    if (tid == 0) s_base = 0.;
+    __syncthreads();
+    int64_t from = 0;
+    bool crossed = false;
+    for (; residual != kRow && from < a.V && !crossed; from += kThreads) {
+      const int64_t x = from + tid;
+      const double w = x < a.V ? weight_at(p, q, kRow, x) : 0.;
+      const double base = s_base;
+      scan(w, ends, shared);
+      if (w > 0.) atomicMax(&s_positive, (int)x);
+      if (w > 0. && base + ends[tid + 1] > threshold) atomicMin(&s_thread, tid);
+      if (tid == 0) s_base = base + ends[kThreads];
+      __syncthreads();
+      crossed = s_thread < kThreads;
+    }
+    if (tid == 0) *out = crossed ? from - kThreads + s_thread : max(s_positive, 0);
+    return;
+  }
+
+  // Where rounding leaves no crossing, it is the last chunk, and in it the
+  // last token, that has any weight.
+  const bool crossed = s_thread < kThreads;
+  if (!crossed && tid == 0) {
+    s_chunk = s_positive;
+    s_base = 0.;
+  }
+  if (crossed && tid == s_thread) {
+    double base = ends[tid];
+    int found = positive;
+    for (int i = c0; i < positive; ++i) {
+      if (base + partial[i] > threshold) {
+        found = i;
+        break;
+      }
+      base += partial[i];
+    }
+    s_chunk = found;
+    s_base = base;
+  }
+  __syncthreads();
+  const int64_t from = (int64_t)s_chunk * kChunk;
+  const double base = s_base;
+  const int n = (int)(min(from + kChunk, a.V) - from);
+  for (int i = tid; i < kChunk; i += kThreads) weights[i] = i < n ? weight_at(p, q, residual, from + i) : 0.;
+  __syncthreads();
+  for (int j = tid; j < n_without; j += kThreads) {
+    const int64_t x = meta[kMetaHead + j] - from;
+    if (x >= 0 && x < n) weights[x] = 0.;
+  }
+  if (tid == 0) {
+    s_thread = kThreads;
+    s_positive = -1;
+  }
+  __syncthreads();
+  // the token in it: each thread has a run of eight
+  constexpr int kRun = kChunk / kThreads;
+  double w[kRun];
+  sum = 0.;
+  positive = -1;
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    w[i] = weights[tid * kRun + i];
+    sum += w[i];
+    if (w[i] > 0.) positive = tid * kRun + i;
+  }
+  scan(sum, ends, shared);
+  if (positive >= 0) atomicMax(&s_positive, positive);
+  if (crossed && positive >= 0 && base + ends[tid + 1] > threshold) atomicMin(&s_thread, tid);
+  __syncthreads();
+  if (s_thread == kThreads) {
+    if (tid == 0) *out = from + max(s_positive, 0);
+  } else if (tid == s_thread) {
+    double at = base + ends[tid];
+    int found = positive;
+#pragma unroll
+    for (int i = kRun - 1; i >= 0; --i) {  // the first is found last
+      double upto = at;
+#pragma unroll
+      for (int j = 0; j <= i; ++j) upto += w[j];
+      if (w[i] > 0. && upto > threshold) found = tid * kRun + i;
+    }
+    *out = from + found;
+  }
+}
+
+template <typename T>
+hipError_t verify_by_type(const VerifyArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((verify_walk_kernel<T>), dim3(a.chunks, a.B), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((verify_answer_kernel<T>), dim3(a.B), dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int verify_chunks(int64_t V) { return (int)((V + kChunk - 1) / kChunk); }
+int verify_max_nodes() { return kMaxNodes; }
+int verify_meta_ints(int T) { return kMetaHead + T; }
+
+hipError_t launch_verify(const VerifyArgs& a, ServingType type, hipStream_t stream) {
+  switch (type) {
+    case ServingType::kBf16: return verify_by_type<__bf16>(a, stream);
+    case ServingType::kFp16: return verify_by_type<_Float16>(a, stream);
+    default: return verify_by_type<float>(a, stream);
+  }
+}
