@@ -9,6 +9,7 @@ on-device trig turns memory-bound kernels VALU-bound).
 
 import math
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -27,6 +28,7 @@ class LlamaConfig:
     rms_norm_eps: float = 1e-5
     rope_theta: float = 500000.0
     tie_word_embeddings: bool = False
+    rope_scaling: Optional[dict] = None  # as ops.rope.rope_frequencies takes it
 
     @classmethod
     def llama3_8b(cls, **overrides):
@@ -62,10 +64,16 @@ class LlamaConfig:
 
 # RMSNorm: the fused CDNA4 kernel (bf16 one-pass fwd, two-kernel bwd) with
 # a built-in eager fallback for CPU / non-bf16 (accelerate_amd.ops.norms)
+from ..ops.kv_cache import KVCache, cache_attention, draft_tree_mask
 from ..ops.norms import FusedRMSNorm as RMSNorm
 
 
-def build_rope_cache(seq_len, head_dim, theta, device, dtype=torch.float32):
+def build_rope_cache(seq_len, head_dim, theta, device, dtype=torch.float32, scaling=None):
+    if scaling is not None:
+        from ..ops.rope import rope_tables
+
+        cos, sin = rope_tables(seq_len, head_dim, theta, scaling, device)
+        return cos.to(dtype), sin.to(dtype)
     inv_freq = 1.0 / (theta ** (torch.arange(0, head_dim, 2, device=device).float() / head_dim))
     t = torch.arange(seq_len, device=device).float()
     freqs = torch.outer(t, inv_freq)
@@ -88,6 +96,19 @@ def apply_rope(x, cos, sin):
     return torch.cat([x1 * cosd - x2 * sind, x2 * cosd + x1 * sind], dim=-1)
 
 
+@dataclass
+class CacheStep:
+    """What a layer needs to run new tokens behind its KVCache: their positions [B, T] in the rotary tables, their
+    slots from the standing tokens on, and which of the new slots each one sees (None: a chain). The first tokens of
+    all (``prefill``) attend each other alone."""
+
+    cache: KVCache
+    positions: torch.Tensor
+    offset: int = 0
+    mask: Optional[torch.Tensor] = None
+    prefill: bool = False
+
+
 class LlamaAttention(nn.Module):
     def __init__(self, config: LlamaConfig, attn_impl: str = "chunked"):
         super().__init__()
@@ -105,6 +126,18 @@ class LlamaAttention(nn.Module):
         q = self.q_proj(x).view(B, S, self.n_heads, self.head_dim).transpose(1, 2)
         k = self.k_proj(x).view(B, S, self.n_kv, self.head_dim).transpose(1, 2)
         v = self.v_proj(x).view(B, S, self.n_kv, self.head_dim).transpose(1, 2)
+        if isinstance(kv_cache, CacheStep):
+            from ..ops.attention import flash_attention
+            from ..ops.rope import rotary_embedding
+
+            step = kv_cache
+            q, k = rotary_embedding(q, k, cos, sin, positions=step.positions)
+            step.cache.append(k, v, offset=step.offset)
+            if step.prefill and S > 1:
+                ctx = flash_attention(q, k, v, causal=True)
+            else:
+                ctx = cache_attention(q, step.cache, mask=step.mask)
+            return self.o_proj(ctx.transpose(1, 2).reshape(B, S, -1))
         # sequence parallelism (CP/Ulysses): x is this rank's sequence shard;
         # RoPE uses the shard's ABSOLUTE positions and the attention runs
         # through the registered collective pattern (ops.attention dispatch)
@@ -210,7 +243,9 @@ class LlamaForCausalLM(nn.Module):
         if c.tie_word_embeddings:
             self.lm_head.weight = self.embed_tokens.weight
         head_dim = c.hidden_size // c.num_attention_heads
-        cos, sin = build_rope_cache(c.max_position_embeddings, head_dim, c.rope_theta, "cpu")
+        cos, sin = build_rope_cache(
+            c.max_position_embeddings, head_dim, c.rope_theta, "cpu", scaling=c.rope_scaling
+        )
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
         self.apply(self._init_weights)
@@ -223,11 +258,22 @@ class LlamaForCausalLM(nn.Module):
         elif isinstance(module, nn.Embedding):
             module.weight.data.normal_(mean=0.0, std=0.02)
 
-    def forward(self, input_ids, labels=None, kv_caches=None):
+    def forward(self, input_ids, labels=None, kv_caches=None, positions=None, mask=None, offset=0, prefill=False):
+        """``kv_caches`` are the dicts of ``make_kv_caches`` or the KVCaches of ``make_serving_caches``. The latter take
+        the tokens behind those that stand (from ``offset`` on, at ``positions`` [B, T], each seeing what ``mask`` says:
+        see ``cache_attention``) and are not advanced; ``prefill`` says that nothing stands yet."""
         x = self.embed_tokens(input_ids)
-        past = kv_caches[0]["len"] if kv_caches is not None else 0
-        cos = self.rope_cos[past:].to(x.device)
-        sin = self.rope_sin[past:].to(x.device)
+        if kv_caches is not None and isinstance(kv_caches[0], KVCache):
+            # a model cast to bf16 has cast its tables too; the kernel reads fp32
+            cos, sin = self.rope_cos.to(x.device).float(), self.rope_sin.to(x.device).float()
+            if positions is None:
+                after = torch.arange(offset, offset + input_ids.shape[1], device=x.device)
+                positions = kv_caches[0].lengths.long()[:, None] + after
+            kv_caches = [CacheStep(cache, positions, offset, mask, prefill) for cache in kv_caches]
+        else:
+            past = kv_caches[0]["len"] if kv_caches is not None else 0
+            cos = self.rope_cos[past:].to(x.device)
+            sin = self.rope_sin[past:].to(x.device)
         for i, layer in enumerate(self.layers):
             x = layer(x, cos, sin, kv_caches[i] if kv_caches is not None else None)
         x = self.norm(x)
@@ -250,6 +296,19 @@ class LlamaForCausalLM(nn.Module):
             }
             for _ in range(c.num_hidden_layers)
         ]
+
+    def make_serving_caches(self, batch_size, max_len, device, dtype, quant=None, lengths=None):
+        """A KVCache a layer (``quant`` None, "int8" or "fp8"); all share one tensor of lengths."""
+        c = self.config
+        caches = []
+        for layer in self.layers:
+            cache = KVCache(
+                batch_size, layer.self_attn.n_kv, max_len, c.hidden_size // c.num_attention_heads,
+                dtype=dtype, quant=quant, device=device, lengths=lengths,
+            )
+            lengths = cache.lengths
+            caches.append(cache)
+        return caches
 
     def _decode_step_static(self, x_tok, pos, caches, arange_cache, rope_dev):
         """One greedy decode step with STATIC shapes and device-tensor
@@ -291,13 +350,36 @@ class LlamaForCausalLM(nn.Module):
         pos.add_(1)
 
     @torch.no_grad()
-    def generate(self, input_ids, max_new_tokens: int = 32, graph_decode=None):
+    def generate(
+        self,
+        input_ids,
+        max_new_tokens: int = 32,
+        graph_decode=None,
+        cache_dtype=None,
+        draft_model=None,
+        draft_widths=(1, 1, 1, 1),
+        temperature: float = 0.0,
+        generator=None,
+    ):
         """Greedy generation. ``graph_decode=True`` captures the decode
         step into a hipGraph (one replay per token, zero host work) — a win
         for small launch-bound models; measured at PARITY-to-slower on 70B
         (decode there is GEMV-bandwidth-bound and capture-mode BLAS picks
         conservative algorithms: benchmarks/decode_ab.py, 38.9 ms eager vs
-        46 ms graphed), so the default stays eager."""
+        46 ms graphed), so the default stays eager.
+
+        ``cache_dtype`` "int8" or "fp8" holds the keys and values of the
+        cache in 8 bits. ``draft_model`` (a LlamaForCausalLM of the same
+        vocabulary) drafts a tree of tokens a step, ``draft_widths[i]``
+        continuations of each node of depth i, which this model verifies in
+        one pass. ``temperature`` above 0 samples (numbers from
+        ``generator``); a draft of widths 1 is sampled then too. Neither the
+        draft nor its shape changes the distribution of what comes out."""
+        if cache_dtype is not None or draft_model is not None or temperature != 0.0:
+            return self._generate_served(
+                input_ids, max_new_tokens, bool(graph_decode), cache_dtype, draft_model, draft_widths, temperature,
+                generator,
+            )
         device = input_ids.device
         dtype = self.lm_head.weight.dtype
         caches = self.make_kv_caches(input_ids.shape[0], input_ids.shape[1] + max_new_tokens, device, dtype)
@@ -344,6 +426,138 @@ class LlamaForCausalLM(nn.Module):
         for c in caches:
             c["len"] = start + max_new_tokens - 1
         return torch.cat(tokens, dim=1)
+
+
+    def _target_probs(self, logits, temperature):
+        """The distributions that tokens are drawn from: of the most likely token alone at temperature 0."""
+        if temperature == 0.0:
+            best = logits.argmax(-1, keepdim=True)
+            return torch.zeros_like(logits).scatter_(-1, best, 1.0)
+        return torch.softmax(logits.float() / temperature, -1)
+
+    def _generate_served(
+        self, input_ids, max_new_tokens, graph_decode, cache_dtype, draft_model, draft_widths, temperature, generator
+    ):
+        from ..ops.speculative import verify_draft
+
+        B, S = input_ids.shape
+        device, dtype = input_ids.device, self.lm_head.weight.dtype
+        table = self.rope_cos.shape[0]
+        if temperature < 0:
+            raise ValueError(f"temperature must not be negative, got {temperature}")
+        if max_new_tokens < 1 or S < 1:
+            raise ValueError("generation needs a prompt and at least one new token")
+        if S + max_new_tokens > table:
+            raise ValueError(f"{S} + {max_new_tokens} tokens, the model has {table} positions")
+        if graph_decode and (draft_model is not None or temperature != 0.0):
+            raise ValueError("graph_decode is for greedy decoding without a draft model")
+        # the tree, breadth first: levels are runs of nodes
+        parents, levels = [-1], [(0, 1)]
+        if draft_model is not None:
+            if draft_model.config.vocab_size != self.config.vocab_size:
+                raise ValueError("the draft model has another vocabulary")
+            if draft_model.rope_cos.shape[0] < S + max_new_tokens:
+                raise ValueError("the draft model has fewer positions")
+            if not draft_widths or min(draft_widths) < 1 or max(draft_widths) > self.config.vocab_size:
+                raise ValueError(f"draft_widths must be between 1 and the vocabulary's size, got {draft_widths}")
+            for width in draft_widths:
+                first, last = levels[-1]
+                parents += [node for node in range(first, last) for _ in range(width)]
+                levels.append((last, len(parents)))
+        nodes = len(parents)
+        chain = nodes == len(levels)
+        sampled = chain and temperature != 0.0 and nodes > 1
+        parents = torch.tensor(parents, device=device)
+        mask = draft_tree_mask(parents)
+        depth = mask.sum(-1) - 1
+
+        caches = self.make_serving_caches(B, S + max_new_tokens + nodes, device, dtype, cache_dtype)
+        lengths = caches[0].lengths
+        draft_caches = []
+        if draft_model is not None:  # what stands is the same for both models
+            draft_caches = draft_model.make_serving_caches(
+                B, S + max_new_tokens + nodes, device, draft_model.lm_head.weight.dtype, cache_dtype, lengths
+            )
+
+        def numbers(n):
+            if temperature == 0.0:
+                return torch.zeros(B, n, device=device)
+            return torch.rand(B, n, device=device, generator=generator)
+
+        def draw(probs):
+            """One token of each distribution [B, V]."""
+            return verify_draft(probs[:, None], root.new_zeros(B, 1), numbers(1)).tokens
+
+        root = input_ids.new_zeros(B, 1)
+        logits = self(input_ids, kv_caches=caches, prefill=True)["logits"][:, -1]
+        root = draw(self._target_probs(logits, temperature))
+        if draft_model is not None:
+            draft_model(input_ids, kv_caches=draft_caches, prefill=True)
+        caches[0].advance(S)
+        said = [[t] for t in root[:, 0].tolist()]
+
+        if graph_decode and device.type == "cuda" and max_new_tokens > 1:
+
+            def step():
+                best = self(root, kv_caches=caches)["logits"].argmax(-1)
+                root.copy_(best)
+                caches[0].advance(1)
+
+            first, start = root.clone(), lengths.clone()
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                step()
+            torch.cuda.current_stream().wait_stream(side)
+            root.copy_(first)
+            lengths.copy_(start)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+            out = [input_ids, first]
+            for _ in range(max_new_tokens - 1):
+                graph.replay()
+                out.append(root.clone())
+            return torch.cat(out, dim=1)
+
+        while min(len(s) for s in said) < max_new_tokens:
+            # positions behind the tables are those of drafts that are cut off in the end
+            positions = lengths.long()[:, None] + depth
+            tokens, drawn = [root], []
+            if draft_model is not None:
+                for i, (first, last) in enumerate(levels):
+                    logits = draft_model(
+                        tokens[-1], kv_caches=draft_caches, mask=mask[first:last, :last], offset=first,
+                        positions=positions[:, first:last].clamp(max=draft_model.rope_cos.shape[0] - 1),
+                    )["logits"]
+                    if last == nodes:
+                        break  # these keys and values are for later steps alone
+                    if sampled:
+                        drawn.append(torch.softmax(logits.float() / temperature, -1))
+                        tokens.append(draw(drawn[-1][:, 0]))
+                    else:
+                        tokens.append(logits.topk(draft_widths[i], -1).indices.flatten(1))
+            tokens = torch.cat(tokens, 1)
+            logits = self(
+                tokens, kv_caches=caches, mask=None if chain else mask, positions=positions.clamp(max=table - 1)
+            )["logits"]
+            verdict = verify_draft(
+                self._target_probs(logits, temperature), tokens, numbers(nodes),
+                draft_probs=torch.cat(drawn, 1) if sampled else None, parents=None if chain else parents,
+            )
+            if not chain:
+                for cache in caches + draft_caches:
+                    cache.keep(verdict.path)
+            counts, new = verdict.counts.tolist(), verdict.tokens.tolist()
+            going = [len(s) < max_new_tokens for s in said]
+            caches[0].advance(torch.tensor([g * (n + 1) for g, n in zip(going, counts)], device=device))
+            for s, g, n, t in zip(said, going, counts, new):
+                if g:
+                    s += t[: n + 1]
+            last = torch.gather(verdict.tokens, 1, verdict.counts[:, None])
+            root = torch.where(torch.tensor(going, device=device)[:, None], last, root)
+        new = torch.tensor([s[:max_new_tokens] for s in said], device=device, dtype=input_ids.dtype)
+        return torch.cat((input_ids, new), dim=1)
 
 
 class LlamaPipelineStage(nn.Module):

@@ -77,7 +77,9 @@ class LlamaMoEForCausalLM(nn.Module):
         self.norm = RMSNorm(c.hidden_size, c.rms_norm_eps)
         self.lm_head = nn.Linear(c.hidden_size, c.vocab_size, bias=False)
         head_dim = c.hidden_size // c.num_attention_heads
-        cos, sin = build_rope_cache(c.max_position_embeddings, head_dim, c.rope_theta, "cpu")
+        cos, sin = build_rope_cache(
+            c.max_position_embeddings, head_dim, c.rope_theta, "cpu", scaling=c.rope_scaling
+        )
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
 
