@@ -50,6 +50,7 @@ template <> struct Operand<_Float16> {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;                // keys a wave takes at a time
 constexpr int kStep = kWaves * kTile;    // keys a workgroup takes at a time
+constexpr int kMaxSplits = 512;
 constexpr float kNegInf = -__builtin_inff();
 
 // the value of the code in byte i of a word, exact
@@ -139,7 +140,7 @@ __device__ void add_odd_row(const AttendArgs& a, int b, int t, int n0, int from,
 }
 
 template <typename T, CacheKind kKind, int kD, int kMT>
-__global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(256, (kMT * kD > 256 || kD == 256 ? 1 : 2)) attend_kernel(AttendArgs a) {
   using Op = Operand<T>;
   using OV = typename Op::V;
   constexpr bool kSame = kKind == CacheKind::kSame;
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
   __shared__ float red_m[kWaves][kMT][16], red_l[kWaves][kMT][16];
   __shared__ int red_odd;
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   // Workgroups go round the 8 XCDs in turn. Those that read the same keys for
   // other rows are 8 apart, so that they share an L2.
@@ -179,19 +180,18 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
   const int rows = a.T * a.rep;
   const int row0 = rb * kMT * 16;
 
-  // the queries, as operands: 8 values of row c
+  // the queries, as operands: 8 values of row c. Rows behind the last repeat
+  // it; no row reaches another's result, and they are not written.
   OV q[kMT][kQK];
 #pragma unroll
   for (int mt = 0; mt < kMT; ++mt) {
-    const int row = row0 + mt * 16 + c;
+    const int row = min(row0 + mt * 16 + c, rows - 1);
     const int t = row / a.rep, head = h * a.rep + row % a.rep;
     const T* src = reinterpret_cast<const T*>(a.q) + b * a.qb + head * a.qh + t * a.qt;
 #pragma unroll
     for (int ds = 0; ds < kQK; ++ds) {
       const int d = kPaired ? (ds / 2) * 64 + g * 16 + (ds & 1) * 8 : ds * 32 + g * 8;
-      OV x = {};
-      if (row < rows) x = *reinterpret_cast<const OV*>(src + d);
-      q[mt][ds] = x;
+      q[mt][ds] = *reinterpret_cast<const OV*>(src + d);
     }
   }
 
@@ -215,34 +215,43 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
   const int first = split * share.steps * kStep + wave * kTile;
   const int stop = min(end, (split + 1) * share.steps * kStep);
 
-  for (int key0 = first; key0 < stop; key0 += kStep) {
-    const uint8_t* kp = kbase + (int64_t)key0 * kRowBytes;
-    const uint8_t* vp = vbase + (int64_t)key0 * kRowBytes;
-    constexpr int kLoad = kSame || kPaired ? 16 : 8;
-    constexpr int kLoads = kPaired ? kQK / 2 : kQK;
-    Raw<kLoad> kraw[2][kLoads];
+  // A tile's keys are loaded while the tile before is exponentiated and
+  // multiplied with its values, its values while its own scores are made: the
+  // registers of one are free when the other's next loads start.
+  constexpr int kLoad = kSame || kPaired ? 16 : 8;
+  constexpr int kLoads = kPaired ? kQK / 2 : kQK;
+  Raw<kLoad> kraw[2][kLoads];
+  Raw<kND * kBytes> vraw[8];
+  f32x4 kscale[2], vscale[2];
+  const auto load_keys = [&](int key0) {
+    const uint8_t* kp = kbase + (int64_t)key0 * kRowBytes + c * kRowBytes + g * kLoad;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        kraw[t][i].load(kp + (t * 16 + c) * kRowBytes + (kSame ? i * 64 : i * 64) + g * kLoad);
-    float ksc[8], vsc[8];
+      for (int i = 0; i < kLoads; ++i) kraw[t][i].load(kp + t * 16 * kRowBytes + i * 64);
     if constexpr (!kSame) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(ks + key0 + t * 16 + g * 4);
-        const f32x4 y = *reinterpret_cast<const f32x4*>(vs + key0 + t * 16 + g * 4);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          ksc[t * 4 + r] = x[r] * a.scale_log2;
-          vsc[t * 4 + r] = y[r];
-        }
-      }
+      for (int t = 0; t < 2; ++t) kscale[t] = *reinterpret_cast<const f32x4*>(ks + key0 + t * 16 + g * 4);
     }
-    Raw<kND * kBytes> vraw[8];
+  };
+  const auto load_values = [&](int key0) {
+    const uint8_t* vp = vbase + (int64_t)key0 * kRowBytes + g * 4 * kRowBytes + c * kND * kBytes;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      vraw[e].load(vp + ((e >> 2) * 16 + g * 4 + (e & 3)) * kRowBytes + c * kND * kBytes);
+    for (int e = 0; e < 8; ++e) vraw[e].load(vp + ((e >> 2) * 16 + (e & 3)) * kRowBytes);
+    if constexpr (!kSame) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) vscale[t] = *reinterpret_cast<const f32x4*>(vs + key0 + t * 16 + g * 4);
+    }
+  };
+  // No load is conditional: a wave without keys, or without more, reads its
+  // last tile or the sequence's first once more, from a cache. Registers that
+  // a branch may leave unwritten were given away by the compiler while they
+  // were in use.
+  const int safe = first < stop ? first : 0;
+  load_keys(safe);
+  load_values(safe);
+  for (int key0 = first; key0 < stop; key0 += kStep) {
+    const int next = key0 + kStep < stop ? key0 + kStep : key0;
 
     // scores
     f32x4 s[kMT][2];
@@ -250,21 +259,32 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
     for (int mt = 0; mt < kMT; ++mt) s[mt][0] = s[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ds = 0; ds < kQK; ++ds) {
+      OV k[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        OV k;
         if constexpr (kSame) {
-          k = __builtin_bit_cast(OV, kraw[t][ds]);
+          k[t] = __builtin_bit_cast(OV, kraw[t][ds]);
         } else {
           const auto& raw = kraw[t][kPaired ? ds / 2 : ds];
           const int w0 = kPaired ? (ds & 1) * 2 : 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) k[i] = (T)decode<kKind>(raw.w[w0 + i / 4], i & 3);
+          for (int i = 0; i < 8; ++i) k[t][i] = (T)decode<kKind>(raw.w[w0 + i / 4], i & 3);
         }
+      }
 #pragma unroll
-        for (int mt = 0; mt < kMT; ++mt) s[mt][t] = Op::mfma(k, q[mt][ds], s[mt][t]);
+      for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[mt][t] = Op::mfma(k[t], q[mt][ds], s[mt][t]);
+    }
+    float ksc[8], vsc[8];
+    if constexpr (!kSame) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ksc[e] = kscale[e >> 2][e & 3] * a.scale_log2;
+        vsc[e] = vscale[e >> 2][e & 3];
       }
     }
+    load_keys(next);
 
     const bool masked = key0 + kTile > n0;  // the tile has slots that some rows do not see
     float p[kMT][8];
@@ -273,17 +293,24 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt) {
       const int t_row = (row0 + mt * 16 + c) / a.rep;
-      const bool valid = row0 + mt * 16 + c < rows;
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[mt][e] = s[mt][e >> 2][e & 3] * (kSame ? a.scale_log2 : ksc[e]);
       if (masked) {
+        // all of a lane's mask values are read at once, from inside the mask
+        const bool chain = a.mask == nullptr;
+        const uint8_t* bits = a.mask + b * a.mb + min(t_row, a.T - 1) * a.mt;
+        uint8_t bit[8] = {};
+        if (!chain && a.W > 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) bit[e] = bits[min(max(key0 + (e >> 2) * 16 + g * 4 + (e & 3) - n0, 0), a.W - 1)];
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int key = key0 + (e >> 2) * 16 + g * 4 + (e & 3);
-          bool sees = key < n0;
-          if (!sees && key < end && valid)
-            sees = a.mask ? a.mask[b * a.mb + t_row * a.mt + (key - n0)] != 0 : key - n0 <= t_row;
-          if (!sees) p[mt][e] = kNegInf;
+          // selects, no branches: an array element written under a lane's own
+          // condition was lost by the compiler
+          const bool sees = (key < n0) | ((key < end) & (chain ? key - n0 <= t_row : bit[e] != 0));
+          p[mt][e] = sees ? p[mt][e] : kNegInf;
         }
       }
       float top = p[mt][0];
@@ -309,7 +336,7 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
       if (masked) {  // slots behind the new tokens hold anything
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (key0 + (e >> 2) * 16 + g * 4 + (e & 3) >= end) vsc[e] = 0.f;
+          vsc[e] = key0 + (e >> 2) * 16 + g * 4 + (e & 3) < end ? vsc[e] : 0.f;
       }
     }
     float unit_scale = 1.f;
@@ -350,7 +377,7 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
         if constexpr (!kSame) {
           x *= vsc[e] * unit_scale;
           // the scale of a token that the row does not see may be anything
-          if (masked && p[mt][e] == 0.f) x = 0.f;
+          x = masked & (p[mt][e] == 0.f) ? 0.f : x;
         }
         pv[mt][e] = (T)x;
       }
@@ -369,7 +396,7 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
             unsigned& x = vraw[e].w[w];
             const unsigned low = (x & kExp) == kExp ? 0xFFFFu : 0u;
             const unsigned high = ((x >> 16) & kExp) == kExp ? 0xFFFF0000u : 0u;
-            odd |= in && (low | high);
+            odd |= in & ((low | high) != 0);
             x = in ? x & ~(low | high) : 0u;
           }
         }
@@ -387,6 +414,7 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
 #pragma unroll
       for (int mt = 0; mt < kMT; ++mt) o[mt][j] = Op::mfma(v, pv[mt], o[mt][j]);
     }
+    load_values(next);
   }
 
   // the four waves' parts of a row, joined
@@ -455,40 +483,66 @@ __global__ void __launch_bounds__(256, (kMT * kD > 256 ? 1 : 2)) attend_kernel(A
   }
 }
 
-// The splits of a row, joined: a workgroup a row, its threads over the D
-// dimensions and, where these are fewer, over the splits.
+// The splits of a row, joined: a workgroup a row. Its threads take four
+// dimensions each and share the splits out, so that few rows of many splits
+// (one long sequence) still have many reads under way.
 template <typename T, int kD>
 __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
-  constexpr int kGroups = 256 / kD;
-  __shared__ float red[kGroups][kD], red_l[kGroups];
-  const int rows = a.T * a.rep;
+  constexpr int kLanes = kD / 4, kGroups = 256 / kLanes;
+  __shared__ f32x4 red[kGroups][kLanes];
+  __shared__ float weight[kMaxSplits], red_m[4], red_l[4];
+  const int rows = a.T * a.rep, tid = threadIdx.x;
   const int bh = blockIdx.x / rows, row = blockIdx.x - bh * rows;
   const int b = bh / a.Hkv, h = bh - b * a.Hkv;
-  const int d = threadIdx.x % kD, group = threadIdx.x / kD;
   const int n0 = clamped_length(a, b);
-  const Share share = share_of(min(n0 + a.W, a.max_len), a.splits);
+  const int active = share_of(min(n0 + a.W, a.max_len), a.splits).active;
   const int64_t at = (int64_t)blockIdx.x * a.splits;
-  float top = kNegInf;
-  for (int s = 0; s < share.active; ++s) top = fmaxf(top, a.part_ml[(at + s) * 2]);
-  const float base = top == kNegInf ? 0.f : top;
-  float y = 0.f, sum = 0.f;
-  for (int s = group; s < share.active; s += kGroups) {
-    const float weight = __builtin_amdgcn_exp2f(a.part_ml[(at + s) * 2] - base);
-    y += a.part_o[(at + s) * kD + d] * weight;
-    sum += a.part_ml[(at + s) * 2 + 1] * weight;
-  }
-  red[group][d] = y;
-  if (d == 0) red_l[group] = sum;
-  __syncthreads();
-  if (group) return;
+
+  float m[kMaxSplits / 256], l[kMaxSplits / 256], top = kNegInf;
 #pragma unroll
-  for (int i = 1; i < kGroups; ++i) {
-    y += red[i][d];
-    sum += red_l[i];
+  for (int i = 0; i < kMaxSplits / 256; ++i) {
+    const int s = tid + i * 256;
+    m[i] = kNegInf;
+    l[i] = 0.f;
+    if (s < active) {
+      m[i] = a.part_ml[(at + s) * 2];
+      l[i] = a.part_ml[(at + s) * 2 + 1];
+    }
+    top = fmaxf(top, m[i]);
   }
+#pragma unroll
+  for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+  if ((tid & 63) == 0) red_m[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+  const float base = top == kNegInf ? 0.f : top;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 256; ++i) {
+    const float w = __builtin_amdgcn_exp2f(m[i] - base);
+    weight[tid + i * 256] = w;
+    sum += l[i] * w;
+  }
+#pragma unroll
+  for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+  if ((tid & 63) == 0) red_l[tid >> 6] = sum;
+  __syncthreads();
+  sum = red_l[0] + red_l[1] + red_l[2] + red_l[3];
+
+  const int lane = tid % kLanes, group = tid / kLanes;
+  const float* part = a.part_o + at * kD + lane * 4;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = group; s < active; s += kGroups) y += *reinterpret_cast<const f32x4*>(part + (int64_t)s * kD) * weight[s];
+  red[group][lane] = y;
+  __syncthreads();
+  if (tid >= kD) return;
+  float out = 0.f;
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) out += red[i][tid / 4][tid % 4];
   const int t = row / a.rep, head = h * a.rep + row % a.rep;
-  const float out = sum == 0.f ? empty_row(a, b, t, n0) : y / sum;
-  reinterpret_cast<T*>(a.out)[b * a.ob + head * a.oh + t * a.ot + d] = (T)out;
+  out = sum == 0.f ? empty_row(a, b, t, n0) : out / sum;
+  reinterpret_cast<T*>(a.out)[b * a.ob + head * a.oh + t * a.ot + tid] = (T)out;
 }
 
 template <typename T, CacheKind kKind, int kD>
@@ -542,7 +596,7 @@ int attend_row_tiles(int rows, int D) {
 // sequence is shared out over the same number, as far as its steps go.
 int attend_splits(const AttendArgs& a) {
   const int64_t groups = (int64_t)a.B * a.Hkv * a.row_blocks;
-  const int64_t wanted = (512 + groups - 1) / groups;
+  const int64_t wanted = (kMaxSplits + groups - 1) / groups;
   const int64_t most = (a.max_len + kStep - 1) / kStep;
   return (int)std::max<int64_t>(1, std::min(wanted, most));
 }

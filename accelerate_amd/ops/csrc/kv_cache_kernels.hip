@@ -11,19 +11,22 @@
 // NaN then, and it reads back as NaN. A row whose int8 scale would be
 // subnormal (amax below 127 * 2^-126) is held as zeros.
 //
-// All of these are bound by memory: a lane holds 8 values (16 bytes of input,
-// 8 of codes), D / 8 lanes hold a row, and a wave 512 / D rows of one head
-// that follow each other, whose codes and scales are one run of memory.
+// All of these are bound by memory, and nearly by the instructions around it:
+// a lane holds 16 values (32 bytes of input, 16 of codes), D / 16 lanes a row,
+// and the grid's y and z are the sequence and the tensor, so that one division
+// finds a row. Rows of a call go over heads first where the input has the
+// heads of a token side by side, so that whole pages of it are read at a time.
 
 #include "serving.h"
 
 namespace {
 
-typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
 typedef unsigned int uint4v __attribute__((ext_vector_type(4)));
 
+constexpr int kPer = 16;  // values a lane
+
 template <typename T>
-struct alignas(16) Eight { T v[8]; };
+struct alignas(16) Values { T v[kPer]; };
 
 constexpr unsigned kInfBits = 0x7F800000u;
 
@@ -68,45 +71,39 @@ __device__ __forceinline__ void values4(unsigned word, float scale, float* y) {
   }
 }
 
-// which tensor, sequence, head and token a row is; tokens run fastest
+// The head and token of a thread's row of its sequence.
 struct Row {
-  int which, b, h, t;
+  int h, t;
 };
 
 __device__ __forceinline__ Row row_of(unsigned row, const CacheArgs& a) {
-  const unsigned per = (unsigned)a.B * a.H * a.T;
-  Row r;
-  r.which = row >= per;
-  unsigned rest = r.which ? row - per : row;
-  unsigned q = rest / (unsigned)a.T;
-  r.t = (int)(rest - q * a.T);
-  r.b = (int)(q / (unsigned)a.H);
-  r.h = (int)(q - (unsigned)r.b * a.H);
-  return r;
+  const unsigned inner = a.heads_first ? a.H : a.T;
+  const unsigned q = row / inner, r = row - q * inner;
+  return a.heads_first ? Row{(int)r, (int)q} : Row{(int)q, (int)r};
 }
 
 template <typename T, CacheKind kKind, int kD>
 __global__ void __launch_bounds__(256) cache_append_kernel(CacheArgs a) {
-  constexpr int kLanes = kD / 8;
-  const int lane = threadIdx.x % kLanes;
+  constexpr int kLanes = kD / kPer;
+  const int lane = threadIdx.x % kLanes, b = blockIdx.y, which = blockIdx.z;
   const unsigned row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  if (row >= 2u * a.B * a.H * a.T) return;  // whole groups of kLanes lanes leave together
+  if (row >= (unsigned)a.H * a.T) return;  // whole groups of kLanes lanes leave together
   const Row r = row_of(row, a);
-  if (a.counts && r.t >= a.counts[r.b]) return;
-  const int64_t slot = (a.start ? (int64_t)a.start[r.b] : 0) + a.offset + r.t;
+  if (a.counts && r.t >= a.counts[b]) return;
+  const int64_t slot = (a.start ? (int64_t)a.start[b] : 0) + a.offset + r.t;
   if (slot < 0 || slot >= a.max_len) return;
-  const T* x = reinterpret_cast<const T*>(a.x[r.which]) + r.b * a.sb[r.which] + r.h * a.sh[r.which] +
-               r.t * a.st[r.which] + lane * 8;
-  const Eight<T> in = *reinterpret_cast<const Eight<T>*>(x);
-  const CacheTensor& out = r.which ? a.v : a.k;
-  const int64_t at = ((int64_t)r.b * a.H + r.h) * a.slots + slot;
+  const T* x = reinterpret_cast<const T*>(a.x[which]) + b * a.sb[which] + r.h * a.sh[which] + r.t * a.st[which] +
+               lane * kPer;
+  const Values<T> in = *reinterpret_cast<const Values<T>*>(x);
+  const CacheTensor& out = which ? a.v : a.k;
+  const int64_t at = ((int64_t)b * a.H + r.h) * a.slots + slot;
   if constexpr (kKind == CacheKind::kSame) {
-    *reinterpret_cast<Eight<T>*>(reinterpret_cast<T*>(out.data) + at * kD + lane * 8) = in;
+    *reinterpret_cast<Values<T>*>(reinterpret_cast<T*>(out.data) + at * kD + lane * kPer) = in;
   } else {
-    float f[8];
+    float f[kPer];
     unsigned most = 0;  // of the absolute values' bits: infinities and NaN are above all others
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kPer; ++i) {
       f[i] = (float)in.v[i];
       most = max(most, __float_as_uint(f[i]) & 0x7FFFFFFFu);
     }
@@ -123,48 +120,50 @@ __global__ void __launch_bounds__(256) cache_append_kernel(CacheArgs a) {
       scale = most ? __uint_as_float((unsigned)(e + 127) << 23) : 0.f;
       inverse = __uint_as_float((unsigned)(127 - e) << 23);
     }
-    uint2v codes = {0u, 0u};
+    uint4v codes = {0u, 0u, 0u, 0u};
     if (most >= kInfBits) {
       scale = __builtin_nanf("");
     } else if (scale > 0.f) {
-      if constexpr (kKind == CacheKind::kInt8) codes = {codes4_int8(f, scale, inverse), codes4_int8(f + 4, scale, inverse)};
-      else codes = {codes4_fp8(f, inverse), codes4_fp8(f + 4, inverse)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kKind == CacheKind::kInt8) codes[i] = codes4_int8(f + 4 * i, scale, inverse);
+        else codes[i] = codes4_fp8(f + 4 * i, inverse);
+      }
     }
-    *reinterpret_cast<uint2v*>(reinterpret_cast<uint8_t*>(out.data) + at * kD + lane * 8) = codes;
+    *reinterpret_cast<uint4v*>(reinterpret_cast<uint8_t*>(out.data) + at * kD + lane * kPer) = codes;
     if (lane == 0) out.scale[at] = scale;
   }
 }
 
 template <typename T, CacheKind kKind, typename Out, int kD>
 __global__ void __launch_bounds__(256) cache_read_kernel(CacheArgs a) {
-  constexpr int kLanes = kD / 8;
-  const int lane = threadIdx.x % kLanes;
+  constexpr int kLanes = kD / kPer;
+  const int lane = threadIdx.x % kLanes, b = blockIdx.y, which = blockIdx.z;
   const unsigned row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  if (row >= 2u * a.B * a.H * a.T) return;
-  const Row r = row_of(row, a);
-  const int64_t slot = (a.start ? (int64_t)a.start[r.b] : 0) + a.offset + r.t;
-  const CacheTensor& in = r.which ? a.v : a.k;
-  const int64_t at = ((int64_t)r.b * a.H + r.h) * a.slots + slot;
-  float f[8] = {};  // slots that the cache does not have read as zeros
+  if (row >= (unsigned)a.H * a.T) return;
+  const Row r = row_of(row, a);  // tokens first, as the output has them
+  const int64_t slot = (a.start ? (int64_t)a.start[b] : 0) + a.offset + r.t;
+  const CacheTensor& in = which ? a.v : a.k;
+  const int64_t at = ((int64_t)b * a.H + r.h) * a.slots + slot;
+  float f[kPer] = {};  // slots that the cache does not have read as zeros
   if (slot >= 0 && slot < a.max_len) {
     if constexpr (kKind == CacheKind::kSame) {
-      const Eight<T> held = *reinterpret_cast<const Eight<T>*>(reinterpret_cast<const T*>(in.data) + at * kD + lane * 8);
+      const Values<T> held = *reinterpret_cast<const Values<T>*>(reinterpret_cast<const T*>(in.data) + at * kD + lane * kPer);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = (float)held.v[i];
+      for (int i = 0; i < kPer; ++i) f[i] = (float)held.v[i];
     } else {
-      const uint2v codes =
-          *reinterpret_cast<const uint2v*>(reinterpret_cast<const uint8_t*>(in.data) + at * kD + lane * 8);
+      const uint4v codes =
+          *reinterpret_cast<const uint4v*>(reinterpret_cast<const uint8_t*>(in.data) + at * kD + lane * kPer);
       const float scale = in.scale[at];
-      values4<kKind>(codes[0], scale, f);
-      values4<kKind>(codes[1], scale, f + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) values4<kKind>(codes[i], scale, f + 4 * i);
     }
   }
-  const unsigned per = (unsigned)a.B * a.H * a.T;
-  Out* y = reinterpret_cast<Out*>(a.y[r.which]) + (int64_t)(r.which ? row - per : row) * kD + lane * 8;
-  Eight<Out> o;
+  Out* y = reinterpret_cast<Out*>(a.y[which]) + ((int64_t)b * a.H * a.T + row) * kD + lane * kPer;
+  Values<Out> o;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o.v[i] = (Out)f[i];
-  *reinterpret_cast<Eight<Out>*>(y) = o;
+  for (int i = 0; i < kPer; ++i) o.v[i] = (Out)f[i];
+  *reinterpret_cast<Values<Out>*>(y) = o;
 }
 
 // The kept tokens of a sequence, in order: slot start + path[i] to start + i.
@@ -194,8 +193,8 @@ __global__ void __launch_bounds__(64) cache_keep_kernel(CacheArgs a, const int64
 
 template <typename T, CacheKind kKind, int kD>
 hipError_t append_launch(const CacheArgs& a, hipStream_t stream) {
-  const unsigned rows = 2u * a.B * a.H * a.T, per = 256 / (kD / 8);
-  hipLaunchKernelGGL((cache_append_kernel<T, kKind, kD>), dim3((rows + per - 1) / per), dim3(256), 0, stream, a);
+  const unsigned rows = (unsigned)a.H * a.T, per = 256 / (kD / kPer);
+  hipLaunchKernelGGL((cache_append_kernel<T, kKind, kD>), dim3((rows + per - 1) / per, a.B, 2), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -211,8 +210,8 @@ hipError_t append_by_dim(const CacheArgs& a, hipStream_t stream) {
 
 template <typename T, CacheKind kKind, typename Out, int kD>
 hipError_t read_launch(const CacheArgs& a, hipStream_t stream) {
-  const unsigned rows = 2u * a.B * a.H * a.T, per = 256 / (kD / 8);
-  hipLaunchKernelGGL((cache_read_kernel<T, kKind, Out, kD>), dim3((rows + per - 1) / per), dim3(256), 0, stream, a);
+  const unsigned rows = (unsigned)a.H * a.T, per = 256 / (kD / kPer);
+  hipLaunchKernelGGL((cache_read_kernel<T, kKind, Out, kD>), dim3((rows + per - 1) / per, a.B, 2), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -44,6 +44,7 @@ struct CacheArgs {
   int64_t offset;          // added to it
   const int* counts;       // [B] tokens that are written, or null: all T
   int B, H, T, D, slots, max_len;
+  int heads_first;         // rows in the order of their heads, then tokens
 };
 
 struct AttendArgs {

@@ -48,7 +48,9 @@ constexpr int64_t kMaxInt = std::numeric_limits<int>::max();
 
 }  // namespace
 
-std::tuple<at::Tensor, OptTensor> rotary(at::Tensor q, OptTensor k, at::Tensor cos_t, at::Tensor sin_t,
+namespace {
+
+std::tuple<at::Tensor, OptTensor> rotate(at::Tensor q, OptTensor k, at::Tensor cos_t, at::Tensor sin_t,
                                          OptTensor positions, bool interleaved, bool inverse) {
   const char* who = "rotary_embedding";
   TORCH_CHECK(q.is_cuda() && q.dim() == 4, who, ": q must be a [B, H, S, D] tensor on the GPU");
@@ -131,6 +133,58 @@ std::tuple<at::Tensor, OptTensor> rotary(at::Tensor q, OptTensor k, at::Tensor c
   return {yq, yk};
 }
 
+// The gradient is the rotation back; being linear, that of the gradient is the
+// rotation itself. In C++, as a Python backward costs more than the kernels of
+// most calls.
+class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, at::Tensor q, OptTensor k,
+                                                at::Tensor cos_t, at::Tensor sin_t, OptTensor positions,
+                                                bool interleaved, bool inverse) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({cos_t, sin_t, positions.value_or(at::Tensor())});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    auto [yq, yk] = rotate(q, k, cos_t, sin_t, positions, interleaved, inverse);
+    if (yk.has_value()) return {yq, *yk};
+    return {yq};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const OptTensor positions = saved[2].defined() ? OptTensor(saved[2]) : OptTensor();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), back = !ctx->saved_data["inverse"].toBool();
+    torch::autograd::variable_list defined, result(7);
+    for (const auto& g : grads)
+      if (g.defined()) defined.push_back(g);
+    if (defined.empty()) return result;
+    const OptTensor second = defined.size() > 1 ? OptTensor(defined[1]) : OptTensor();
+    if (at::GradMode::is_enabled()) {
+      defined = apply(defined[0], second, saved[0], saved[1], positions, interleaved, back);
+    } else {
+      auto [yq, yk] = rotate(defined[0], second, saved[0], saved[1], positions, interleaved, back);
+      defined[0] = yq;
+      if (yk.has_value()) defined[1] = *yk;
+    }
+    size_t next = 0;
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (grads[i].defined()) result[i] = defined[next++];
+    return result;
+  }
+};
+
+}  // namespace
+
+std::tuple<at::Tensor, OptTensor> rotary(at::Tensor q, OptTensor k, at::Tensor cos_t, at::Tensor sin_t,
+                                         OptTensor positions, bool interleaved) {
+  if (at::GradMode::is_enabled() && (q.requires_grad() || (k.has_value() && k->requires_grad()))) {
+    auto y = RotaryFunction::apply(q, k, cos_t, sin_t, positions, interleaved, false);
+    return {y[0], y.size() > 1 ? OptTensor(y[1]) : OptTensor()};
+  }
+  return rotate(q, k, cos_t, sin_t, positions, interleaved, false);
+}
+
 namespace {
 
 // The cache's storage, as KVCache allocates it.
@@ -161,6 +215,7 @@ Cache check_cache(const at::Tensor& k, const at::Tensor& v, const OptTensor& k_s
   TORCH_CHECK(c.D == 32 || c.D == 64 || c.D == 128 || c.D == 256, who, ": head_dim must be 32, 64, 128 or 256, got ", c.D);
   TORCH_CHECK(c.slots % kSlotTile == 0 && max_len >= 0 && max_len <= c.slots && max_len < kMaxInt - 1024, who,
               ": bad slots for max_len ", max_len);
+  TORCH_CHECK(c.B <= 65535, who, ": at most 65535 sequences");
   TORCH_CHECK(aligned16(k) && aligned16(v), who, ": the cache must be aligned to 16 bytes");
   if (c.kind != CacheKind::kSame) {
     for (const OptTensor* s : {&k_scale, &v_scale}) {
@@ -231,6 +286,7 @@ void kv_cache_append(at::Tensor cache_k, at::Tensor cache_v, OptTensor k_scale, 
     a.sh[i] = in[i].stride(1);
     a.st[i] = in[i].stride(2);
   }
+  a.heads_first = a.sh[0] < a.st[0];
   check_launch(launch_cache_append(a, type, c.kind, current_stream()), who);
 }
 
@@ -316,6 +372,7 @@ at::Tensor kv_cache_attend(at::Tensor q, at::Tensor cache_k, at::Tensor cache_v,
   // where the model reshapes [B, T, Hq * D] next, this is a view
   auto out = at::empty({c.B, T, Hq, c.D}, q.options()).transpose(1, 2);
   if (out.numel() == 0) return out;
+  if (max_len == 0 && mask.has_value()) return out.zero_();  // nothing to see
   TORCH_CHECK(T <= max_len || mask.has_value(), who, ": ", T, " new tokens, the cache has ", max_len, " slots");
   TORCH_CHECK(c.B * Hq * T < kMaxInt && T * a.rep < kMaxInt, who, ": too many rows");
   q = rows16(q);

@@ -28,7 +28,8 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 2048;     // vocabulary entries a workgroup sums
+constexpr int kRun = 8;           // vocabulary entries a thread sums,
+constexpr int kChunk = kRun * kThreads;  // and a workgroup
 constexpr int kMaxNodes = 1024;  // of a tree, root included
 
 template <typename T>
@@ -45,6 +46,30 @@ enum Residual { kRow = 0, kLess = 1, kWithout = 2 };
 // meta of a sequence: last node, residual, tokens left out, those tokens
 constexpr int kMetaHead = 3;
 
+// A thread's weights x = from, from + kThreads, ...: all reads before their use.
+template <typename T>
+__device__ __forceinline__ void weights_at(const T* p, const T* q, int residual, int64_t from, int64_t to, double* w) {
+  T pv[kRun], qv[kRun];
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    const int64_t x = from + i * kThreads;
+    pv[i] = x < to ? p[x] : (T)0.f;
+    qv[i] = (T)0.f;
+  }
+  if (residual == kLess) {
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int64_t x = from + i * kThreads;
+      if (x < to) qv[i] = q[x];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    const double y = wide(pv[i]) - wide(qv[i]);
+    w[i] = y > 0. ? y : 0.;  // NaN too
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ double weight_at(const T* p, const T* q, int residual, int64_t x) {
   double w = wide(p[x]);
@@ -54,7 +79,7 @@ __device__ __forceinline__ double weight_at(const T* p, const T* q, int residual
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
-  __shared__ double p_of[kMaxNodes], q_of[kMaxNodes];
+  __shared__ double p_of[kMaxNodes], test_of[kMaxNodes];  // taken iff test (times what is left) < p
   __shared__ int token_of[kMaxNodes], parent_of[kMaxNodes], without[kMaxNodes];
   __shared__ int path[kMaxNodes];
   __shared__ int s_last, s_residual, s_without, s_count, s_first;
@@ -72,14 +97,14 @@ __global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
     token_of[i] = is ? (int)token : -1;
     parent_of[i] = is ? (int)parent : -1;
     p_of[i] = is ? wide(target[parent * a.tt + token]) : 0.;
-    q_of[i] = is && draft ? wide(draft[parent * a.dt + token]) : 0.;
+    const double u = uniform_at(a, b, i);
+    test_of[i] = is && draft ? u * wide(draft[parent * a.dt + token]) : u;
   }
   __syncthreads();
 
   if (!a.parents) {  // a chain ends at the first node that is none or not taken
     for (int i = 1 + tid; i < a.T; i += kThreads) {
-      const double u = uniform_at(a, b, i);
-      const bool taken = token_of[i] >= 0 && (draft ? u * q_of[i] < p_of[i] : u < p_of[i]);
+      const bool taken = token_of[i] >= 0 && test_of[i] < p_of[i];
       if (!taken) atomicMin(&s_first, i);
     }
     __syncthreads();
@@ -103,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
       bool again = false;  // a token refused before has nothing left
       for (int j = 0; j < n; ++j) again |= without[j] == token_of[i];
       if (again) continue;
-      if (uniform_at(a, b, i) * left < p_of[i]) {
+      if (test_of[i] * left < p_of[i]) {
         cur = i;
         n = 0;
         left = 1.;
@@ -139,13 +164,15 @@ __global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
   const T* p = target + last * a.tt;
   const T* q = residual == kLess ? draft + last * a.dt : nullptr;
   const int64_t from = (int64_t)chunk * kChunk, to = min(from + kChunk, a.V);
-  double sum = 0.;
-  for (int64_t x = from + tid; x < to; x += kThreads) {
-    double w = weight_at(p, q, residual, x);
-    for (int j = 0; j < n_without; ++j)
-      if (without[j] == x) w = 0.;
-    sum += w;
+  double w[kRun], sum = 0.;
+  weights_at(p, q, residual, from + tid, to, w);
+  for (int j = 0; j < n_without; ++j) {
+#pragma unroll
+    for (int i = 0; i < kRun; ++i)
+      if (without[j] == from + tid + i * kThreads) w[i] = 0.;
   }
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) sum += w[i];
 #pragma unroll
   for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
   if ((tid & 63) == 0) sums[tid >> 6] = sum;
@@ -258,7 +285,10 @@ __global__ void __launch_bounds__(kThreads) verify_answer_kernel(VerifyArgs a) {
   const int64_t from = (int64_t)s_chunk * kChunk;
   const double base = s_base;
   const int n = (int)(min(from + kChunk, a.V) - from);
-  for (int i = tid; i < kChunk; i += kThreads) weights[i] = i < n ? weight_at(p, q, residual, from + i) : 0.;
+  double w[kRun];
+  weights_at(p, q, residual, from + tid, from + n, w);
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) weights[tid + i * kThreads] = w[i];
   __syncthreads();
   for (int j = tid; j < n_without; j += kThreads) {
     const int64_t x = meta[kMetaHead + j] - from;
@@ -270,8 +300,6 @@ __global__ void __launch_bounds__(kThreads) verify_answer_kernel(VerifyArgs a) {
   }
   __syncthreads();
   // the token in it: each thread has a run of eight
-  constexpr int kRun = kChunk / kThreads;
-  double w[kRun];
   sum = 0.;
   positive = -1;
 #pragma unroll

@@ -105,7 +105,7 @@ def rope_tables(max_len: int, rotary_dim: int, theta: float = 10000.0, scaling: 
     return (angle.cos() * factor).float(), (angle.sin() * factor).float()
 
 
-def _rotary_reference(q, k, cos, sin, positions, interleaved, inverse):
+def _rotary_reference(q, k, cos, sin, positions, interleaved):
     def need(ok, message):
         if not ok:
             raise RuntimeError(f"rotary_embedding: {message}")
@@ -138,8 +138,6 @@ def _rotary_reference(q, k, cos, sin, positions, interleaved, inverse):
         at = at.clamp(0, max(cos.shape[0] - 1, 0))
         c = torch.where(known, cos[at][:, None], float("nan"))
         s = torch.where(known, sin[at][:, None], float("nan"))
-    if inverse:
-        s = -s
 
     def rotate(x):
         wide = x.to(torch.promote_types(x.dtype, torch.float32))
@@ -148,33 +146,6 @@ def _rotary_reference(q, k, cos, sin, positions, interleaved, inverse):
         return torch.cat((y, wide[..., 2 * half :]), -1).to(x.dtype)
 
     return rotate(q), None if k is None else rotate(k)
-
-
-def _rotary(q, k, cos, sin, positions, interleaved, inverse):
-    if q.is_cuda:
-        return _load_extension(required=True).rotary(q, k, cos, sin, positions, interleaved, inverse)
-    return _rotary_reference(q, k, cos, sin, positions, interleaved, inverse)
-
-
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(cos, sin, positions)
-        ctx.meta = (interleaved, inverse)
-        return _rotary(q, k, cos, sin, positions, interleaved, inverse)
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        cos, sin, positions = ctx.saved_tensors
-        interleaved, inverse = ctx.meta
-        if dq is None and dk is None:
-            return (None,) * 7
-        if dq is None:
-            dk, _ = _RotaryFn.apply(dk, None, cos, sin, positions, interleaved, not inverse)
-        else:
-            dq, dk = _RotaryFn.apply(dq, dk, cos, sin, positions, interleaved, not inverse)
-        return dq, dk, None, None, None, None, None
 
 
 def rotary_embedding(
@@ -194,8 +165,8 @@ def rotary_embedding(
     have gets NaN in its rotated elements. bf16, fp16 and fp32, any strides (transposed views are read in
     place). The gradient of q and k is the rotation back; the tables have none.
     """
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        out = _RotaryFn.apply(q, k, cos, sin, positions, interleaved, False)
+    if q.is_cuda:
+        out = _load_extension(required=True).rotary(q, k, cos, sin, positions, interleaved)
     else:
-        out = _rotary(q, k, cos, sin, positions, interleaved, False)
+        out = _rotary_reference(q, k, cos, sin, positions, interleaved)
     return out[0] if k is None else out

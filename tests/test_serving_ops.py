@@ -1030,3 +1030,25 @@ def test_other_streams():
     for out in results:
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+@gpu
+def test_rotary_second_gradient():
+    """Of sum(w * grad): the rotation is its own gradient's gradient."""
+    cos, sin = rope_tables(16, 8, device="cuda")
+    q, k = randn(1, 2, 5, 8, device="cuda").requires_grad_(), randn(1, 1, 5, 8, seed=1, device="cuda").requires_grad_()
+    dq, dk = randn(1, 2, 5, 8, seed=2, device="cuda").requires_grad_(), randn(1, 1, 5, 8, seed=3, device="cuda").requires_grad_()
+    gq, gk = torch.autograd.grad(rotary_embedding(q, k, cos, sin), (q, k), (dq, dk), create_graph=True)
+    w = randn(1, 2, 5, 8, seed=4, device="cuda")
+    (second,) = torch.autograd.grad((gq * w).sum(), dq)
+    check_rotated(second, w, cos, sin, None, False)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_cache_without_slots_gives_zeros(device):
+    cache = KVCache(2, 1, 0, 32, dtype=BF16, device=device)
+    mask = torch.zeros(3, 0, dtype=torch.bool, device=device)
+    q = torch.ones(2, 2, 3, 32, dtype=BF16, device=device)
+    assert not cache_attention(q, cache, mask=mask).any()
+    with pytest.raises(RuntimeError):
+        cache_attention(q, cache)
