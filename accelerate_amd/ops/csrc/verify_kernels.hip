@@ -77,18 +77,36 @@ __device__ __forceinline__ double weight_at(const T* p, const T* q, int residual
   return w > 0. ? w : 0.;  // NaN too
 }
 
+// The first (last) thread of the workgroup for which a condition holds, or
+// kThreads (-1). By votes: an atomic of all threads is done a lane at a time.
+__device__ __forceinline__ int first_thread(bool is, int* votes) {
+  const unsigned long long lanes = __ballot(is);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) votes[wave] = lanes ? wave * 64 + __builtin_ctzll(lanes) : kThreads;
+  __syncthreads();
+  return min(min(votes[0], votes[1]), min(votes[2], votes[3]));
+}
+
+__device__ __forceinline__ int last_thread(bool is, int* votes) {
+  const unsigned long long lanes = __ballot(is);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) votes[wave] = lanes ? wave * 64 + 63 - __builtin_clzll(lanes) : -1;
+  __syncthreads();
+  return max(max(votes[0], votes[1]), max(votes[2], votes[3]));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
   __shared__ double p_of[kMaxNodes], test_of[kMaxNodes];  // taken iff test (times what is left) < p
   __shared__ int token_of[kMaxNodes], parent_of[kMaxNodes], without[kMaxNodes];
   __shared__ int path[kMaxNodes];
-  __shared__ int s_last, s_residual, s_without, s_count, s_first;
+  __shared__ int s_last, s_residual, s_without, s_count;
+  __shared__ int votes[2][kThreads / 64];
   __shared__ double sums[kThreads / 64];
   const int b = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
   const T* target = reinterpret_cast<const T*>(a.target) + b * a.tb;
   const T* draft = a.draft ? reinterpret_cast<const T*>(a.draft) + b * a.db : nullptr;
 
-  if (tid == 0) s_first = a.T;
   for (int i = tid; i < a.T; i += kThreads) {
     const int64_t token = a.tokens[b * a.kb + i];
     const int64_t parent = i == 0 ? -1 : (a.parents ? a.parents[b * a.pb + i] : (int64_t)i - 1);
@@ -103,21 +121,22 @@ __global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
   __syncthreads();
 
   if (!a.parents) {  // a chain ends at the first node that is none or not taken
-    for (int i = 1 + tid; i < a.T; i += kThreads) {
-      const bool taken = token_of[i] >= 0 && test_of[i] < p_of[i];
-      if (!taken) atomicMin(&s_first, i);
+    int first = a.T;
+    for (int from = 1; from < a.T && first == a.T; from += kThreads) {
+      const int i = from + tid;
+      const int thread = first_thread(i < a.T && !(token_of[i] >= 0 && test_of[i] < p_of[i]), votes[from / kThreads & 1]);
+      if (thread < kThreads) first = from + thread;
     }
-    __syncthreads();
     if (tid == 0) {
-      const int last = s_first - 1;
-      const bool refused = s_first < a.T && token_of[s_first] >= 0;
+      const int last = first - 1;
+      const bool refused = first < a.T && token_of[first] >= 0;
       s_last = last;
       s_count = last;
       s_residual = !refused ? kRow : draft ? kLess : kWithout;
       s_without = refused && !draft ? 1 : 0;
-      if (s_without) without[0] = token_of[s_first];
+      if (s_without) without[0] = token_of[first];
     }
-    for (int i = tid; i < s_first; i += kThreads) path[i] = i;
+    for (int i = tid; i < first; i += kThreads) path[i] = i;
   } else if (tid == 0) {
     // children come after their parents, so one pass in order is the walk
     int cur = 0, n = 0, count = 0;
@@ -200,22 +219,19 @@ __device__ __forceinline__ void scan(double x, double* ends, double* shared) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_answer_kernel(VerifyArgs a) {
-  __shared__ double weights[kChunk];
+  __shared__ double weights[kChunk + kThreads];  // a gap after each thread's run: no two start in one bank
   __shared__ double ends[kThreads + 1], shared[kThreads / 64];
   __shared__ double s_base;
-  __shared__ int s_thread, s_chunk, s_positive;
+  __shared__ int s_chunk, votes[6][kThreads / 64];
   const int b = blockIdx.x, tid = threadIdx.x;
   const int* meta = a.meta + (int64_t)b * (kMetaHead + a.T);
   const int last = meta[0], residual = meta[1], n_without = meta[2];
+  const int gone = tid < n_without ? meta[kMetaHead + tid] : 0;  // read while the sums are
   const T* p = reinterpret_cast<const T*>(a.target) + b * a.tb + last * a.tt;
   const T* q = residual == kLess ? reinterpret_cast<const T*>(a.draft) + b * a.db + last * a.dt : nullptr;
   int64_t* out = a.out_tokens + (int64_t)b * a.T + a.counts[b];
   const double u = fmax(uniform_at(a, b, 0), 0.);
   const double* partial = a.partial + (int64_t)b * a.chunks;
-  if (tid == 0) {
-    s_thread = kThreads;
-    s_positive = -1;
-  }
 
   // the chunk: each thread has a run of them
   const int per = (a.chunks + kThreads - 1) / kThreads;
@@ -227,12 +243,11 @@ __global__ void __launch_bounds__(kThreads) verify_answer_kernel(VerifyArgs a) {
     if (partial[i] > 0.) positive = i;
   }
   scan(sum, ends, shared);
-  if (positive >= 0) atomicMax(&s_positive, positive);
   double threshold = u * ends[kThreads];
-  if (ends[tid + 1] > threshold && positive >= 0) atomicMin(&s_thread, tid);
-  __syncthreads();
+  const int passing = first_thread(ends[tid + 1] > threshold && positive >= 0, votes[0]);
+  const int last_positive = last_thread(positive >= 0, votes[1]);
 
-  if (s_positive < 0) {
+  if (last_positive < 0) {
     // No weight at all. A residual that has none (a draft that covered all of
     // the target) gives way to the row itself; that, to token 0. Rare: the
     // whole workgroup goes over the row, twice.
@@ -242,36 +257,32 @@ __global__ void __launch_bounds__(kThreads) verify_answer_kernel(VerifyArgs a) {
     __syncthreads();
     scan(row, ends, shared);
     threshold = u * ends[kThreads];
-    if (tid == 0) s_base = 0.;
-    __syncthreads();
-    int64_t from = 0;
+    int64_t token = 0;
     bool crossed = false;
-    for (; residual != kRow && from < a.V && !crossed; from += kThreads) {
+    double base = 0.;
+    for (int64_t from = 0; residual != kRow && from < a.V && !crossed; from += kThreads) {
       const int64_t x = from + tid;
       const double w = x < a.V ? weight_at(p, q, kRow, x) : 0.;
-      const double base = s_base;
-      scan(w, ends, shared);
-      if (w > 0.) atomicMax(&s_positive, (int)x);
-      if (w > 0. && base + ends[tid + 1] > threshold) atomicMin(&s_thread, tid);
-      if (tid == 0) s_base = base + ends[kThreads];
       __syncthreads();
-      crossed = s_thread < kThreads;
+      scan(w, ends, shared);
+      const int thread = first_thread(w > 0. && base + ends[tid + 1] > threshold, votes[2]);
+      const int some = last_thread(w > 0., votes[3]);
+      crossed = thread < kThreads;
+      if (crossed) token = from + thread;
+      else if (some >= 0) token = from + some;
+      base += ends[kThreads];
     }
-    if (tid == 0) *out = crossed ? from - kThreads + s_thread : max(s_positive, 0);
+    if (tid == 0) *out = token;
     return;
   }
 
   // Where rounding leaves no crossing, it is the last chunk, and in it the
   // last token, that has any weight.
-  const bool crossed = s_thread < kThreads;
-  if (!crossed && tid == 0) {
-    s_chunk = s_positive;
-    s_base = 0.;
-  }
-  if (crossed && tid == s_thread) {
+  const bool crossed = passing < kThreads;
+  if (tid == (crossed ? passing : last_positive)) {
     double base = ends[tid];
     int found = positive;
-    for (int i = c0; i < positive; ++i) {
+    for (int i = c0; crossed && i < positive; ++i) {
       if (base + partial[i] > threshold) {
         found = i;
         break;
@@ -288,15 +299,11 @@ __global__ void __launch_bounds__(kThreads) verify_answer_kernel(VerifyArgs a) {
   double w[kRun];
   weights_at(p, q, residual, from + tid, from + n, w);
 #pragma unroll
-  for (int i = 0; i < kRun; ++i) weights[tid + i * kThreads] = w[i];
+  for (int i = 0; i < kRun; ++i) weights[tid + i * kThreads + (tid + i * kThreads) / kRun] = w[i];
   __syncthreads();
   for (int j = tid; j < n_without; j += kThreads) {
-    const int64_t x = meta[kMetaHead + j] - from;
-    if (x >= 0 && x < n) weights[x] = 0.;
-  }
-  if (tid == 0) {
-    s_thread = kThreads;
-    s_positive = -1;
+    const int64_t x = (j < kThreads ? gone : meta[kMetaHead + j]) - from;
+    if (x >= 0 && x < n) weights[x + x / kRun] = 0.;
   }
   __syncthreads();
   // the token in it: each thread has a run of eight
@@ -304,17 +311,16 @@ __global__ void __launch_bounds__(kThreads) verify_answer_kernel(VerifyArgs a) {
   positive = -1;
 #pragma unroll
   for (int i = 0; i < kRun; ++i) {
-    w[i] = weights[tid * kRun + i];
+    w[i] = weights[tid * (kRun + 1) + i];
     sum += w[i];
     if (w[i] > 0.) positive = tid * kRun + i;
   }
   scan(sum, ends, shared);
-  if (positive >= 0) atomicMax(&s_positive, positive);
-  if (crossed && positive >= 0 && base + ends[tid + 1] > threshold) atomicMin(&s_thread, tid);
-  __syncthreads();
-  if (s_thread == kThreads) {
-    if (tid == 0) *out = from + max(s_positive, 0);
-  } else if (tid == s_thread) {
+  const int holder = first_thread(crossed && positive >= 0 && base + ends[tid + 1] > threshold, votes[4]);
+  const int final = last_thread(positive >= 0, votes[5]);
+  if (holder == kThreads) {  // rounding left no crossing in it
+    if (tid == max(final, 0)) *out = from + max(positive, 0);
+  } else if (tid == holder) {
     double at = base + ends[tid];
     int found = positive;
 #pragma unroll
