@@ -33,15 +33,19 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int uint4v __attribute__((ext_vector_type(4)));
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 template <typename T> struct Operand;
 template <> struct Operand<__bf16> {
   typedef __bf16 V __attribute__((ext_vector_type(8)));
+  typedef __bf16 Pair __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
 };
 template <> struct Operand<_Float16> {
   typedef _Float16 V __attribute__((ext_vector_type(8)));
+  typedef _Float16 Pair __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -50,19 +54,51 @@ template <> struct Operand<_Float16> {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;                // keys a wave takes at a time
 constexpr int kStep = kWaves * kTile;    // keys a workgroup takes at a time
-constexpr int kMaxSplits = 512;
+constexpr int kMaxSplits = 512, kFewSplits = 8;
 constexpr float kNegInf = -__builtin_inff();
+constexpr float kNothing = -0x1p127f;  // the maximum of no scores: finite, so that its difference to them is a number
 
-// the value of the code in byte i of a word, exact
-template <CacheKind kKind>
-__device__ __forceinline__ float decode(unsigned word, int i) {
-  if constexpr (kKind == CacheKind::kInt8) return (float)(int8_t)(word >> (8 * i));
-  switch (i) {  // the byte is an immediate of the instruction
-    case 0: return __builtin_amdgcn_cvt_f32_fp8(word, 0);
-    case 1: return __builtin_amdgcn_cvt_f32_fp8(word, 1);
-    case 2: return __builtin_amdgcn_cvt_f32_fp8(word, 2);
-    default: return __builtin_amdgcn_cvt_f32_fp8(word, 3);
-  }
+// Two values as a word of an operand. (Values that are converted one by one
+// are put together by two instructions more.)
+template <typename T>
+__device__ __forceinline__ unsigned pack2(float x, float y) {
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x, y}, typename Operand<T>::Pair));
+}
+
+// The codes of the two low or high bytes of a word, exact; e4m3 times a power
+// of two.
+template <typename T, CacheKind kKind, bool kHigh>
+__device__ __forceinline__ unsigned decode2(unsigned word, float scale = 1.f) {
+  if constexpr (kKind == CacheKind::kInt8)
+    return pack2<T>((float)(int8_t)(word >> (kHigh ? 16 : 0)), (float)(int8_t)(word >> (kHigh ? 24 : 8)));
+  else if constexpr (__is_same(T, __bf16))
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, kHigh));
+  else
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, scale, kHigh));
+}
+
+// The codes of byte j of two words.
+template <typename T, CacheKind kKind>
+__device__ __forceinline__ unsigned decode_bytes(unsigned a, unsigned b, int j) {
+  if constexpr (kKind == CacheKind::kInt8) return pack2<T>((float)(int8_t)(a >> (8 * j)), (float)(int8_t)(b >> (8 * j)));
+  else return decode2<T, kKind, false>(__builtin_amdgcn_perm(b, a, 0x0400u + 0x0101u * j));
+}
+
+// The largest of a value over the lanes c + 16 g of a row; and the sum.
+template <typename F>
+__device__ __forceinline__ float over_groups(float x, F f) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float max_over_groups(float x) {
+  return over_groups(x, [](float a, float b) { return fmaxf(a, b); });
+}
+
+__device__ __forceinline__ float sum_over_groups(float x) {
+  return over_groups(x, [](float a, float b) { return a + b; });
 }
 
 // bytes of a lane's neighbours in one row, as words (a 2-byte one in the low half)
@@ -91,28 +127,22 @@ struct Raw {
       }
     }
   }
-  template <typename T>
-  __device__ __forceinline__ T as16(int i) const {  // the i-th 16-bit element
-    return __builtin_bit_cast(T, (uint16_t)(w[i / 2] >> (16 * (i & 1))));
-  }
 };
 
 __device__ __forceinline__ int clamped_length(const AttendArgs& a, int b) {
   return min(max(a.lengths[b], 0), a.max_len);
 }
 
-// how many splits of the grid have keys, and how many steps of kStep each has:
-// the sequence's own length is shared out, not the cache's
+// how many splits of the grid have keys, and how many each has: the sequence's
+// own length is shared out in steps of a workgroup's keys, not the cache's
 struct Share {
-  int steps, active;
+  int keys, active;
 };
 
-__device__ __forceinline__ Share share_of(int end, int splits) {
+__device__ __forceinline__ Share share_of(int end, const AttendArgs& a) {
   const int all = max(1, (end + kStep - 1) / kStep);
-  Share s;
-  s.steps = (all + splits - 1) / splits;
-  s.active = (all + s.steps - 1) / s.steps;
-  return s;
+  const int steps = (all + a.splits - 1) / a.splits;
+  return {steps * kStep, (all + steps - 1) / steps};
 }
 
 // A row whose probabilities sum to zero saw nothing and is zero, or all that
@@ -126,364 +156,506 @@ __device__ __forceinline__ float empty_row(const AttendArgs& a, int b, int t, in
   return any ? __builtin_nanf("") : 0.f;
 }
 
-// The infinite and NaN values that the masked tiles left out, of the slots
-// [from, to) that row t sees, added to its sums of N dimensions from d on.
-template <typename T, int N>
-__device__ void add_odd_row(const AttendArgs& a, int b, int t, int n0, int from, int to,
-                                         const uint8_t* values, int d, float* y) {
-  for (int j = max(from, n0 / kTile * kTile); j < to; ++j) {
-    if (j >= n0 && !(a.mask ? a.mask[b * a.mb + t * a.mt + (j - n0)] != 0 : j - n0 <= t)) continue;
-    const T* v = reinterpret_cast<const T*>(values) + (int64_t)j * a.D + d;
-    for (int i = 0; i < N; ++i)
-      if (!__builtin_isfinite((float)v[i])) y[i] += (float)v[i];
+// What a workgroup works on: a split of one sequence's and head's keys, and a
+// block of rows. Workgroups go round the 8 XCDs in turn; those that read the
+// same keys for other rows are 8 apart, so that they share an L2.
+struct Work {
+  int split, bh, b, h, rb, n0, end, from, stop;
+  bool any;
+};
+
+__device__ __forceinline__ Work work_of(const AttendArgs& a) {
+  Work w;
+  const int parts = a.splits * a.Hkv * a.B;
+  int part = blockIdx.x;
+  w.rb = 0;
+  if (a.row_blocks > 1) {
+    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    w.rb = at % a.row_blocks;
+    part = (at / a.row_blocks) * 8 + xcd;
   }
+  w.any = part < parts;
+  w.split = part % a.splits;
+  w.bh = w.any ? part / a.splits : 0;
+  w.b = w.bh / a.Hkv;
+  w.h = w.bh - w.b * a.Hkv;
+  w.n0 = clamped_length(a, w.b);
+  w.end = min(w.n0 + a.W, a.max_len);
+  const Share share = share_of(w.end, a);
+  w.any = w.any && w.split < share.active;
+  w.from = w.split * share.keys;
+  w.stop = min(w.end, w.from + share.keys);
+  return w;
 }
 
-template <typename T, CacheKind kKind, int kD, int kMT>
-__global__ void __launch_bounds__(256, (kMT * kD > 256 || kD == 256 ? 1 : 2)) attend_kernel(AttendArgs a) {
-  using Op = Operand<T>;
-  using OV = typename Op::V;
-  constexpr bool kSame = kKind == CacheKind::kSame;
-  constexpr int kBytes = kSame ? 2 : 1;
-  constexpr int kQK = kD / 32;  // products a tile of 16 keys
-  constexpr int kND = kD / 16;  // a lane's neighbours of a row of V, and products
+template <typename T, CacheKind kKind, int kD>
+struct Shape {
+  static constexpr bool kSame = kKind == CacheKind::kSame;
+  // e4m3 codes times their scale, a power of two, are exact in bf16's range.
+  // Other scales multiply scores and probabilities, in 32 bits.
+  static constexpr bool kFolded = kKind == CacheKind::kFp8 && __is_same(T, __bf16);
+  static constexpr bool kScaled = !kSame && !kFolded;
+  static constexpr int kBytes = kSame ? 2 : 1;
+  static constexpr int kRowBytes = kD * kBytes;
+  static constexpr int kQK = kD / 32;  // products a tile of 16 keys
+  static constexpr int kND = kD / 16;  // a lane's neighbours of a row of V, and products
   // 8-bit keys are loaded 16 values at a time, the two halves of which belong
   // to two products; the queries follow that order
-  constexpr bool kPaired = !kSame && kD >= 64;
-  constexpr int kRowBytes = kD * kBytes;
-  __shared__ float red[kWaves][4][kND][64];
-  __shared__ float red_m[kWaves][kMT][16], red_l[kWaves][kMT][16];
-  __shared__ int red_odd;
+  static constexpr bool kPaired = !kSame && kD >= 64;
+  static constexpr unsigned kExp = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;  // of an infinity or NaN
+};
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  // Workgroups go round the 8 XCDs in turn. Those that read the same keys for
-  // other rows are 8 apart, so that they share an L2.
-  const int parts = a.splits * a.Hkv * a.B;
-  int part, rb;
-  if (a.row_blocks == 1) {
-    part = blockIdx.x;
-    rb = 0;
-  } else {
-    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
-    rb = at % a.row_blocks;
-    part = (at / a.row_blocks) * 8 + xcd;
-    if (part >= parts) return;
-  }
-  const int split = part % a.splits;
-  const int bh = part / a.splits;
-  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
-  const int n0 = clamped_length(a, b);
-  const int end = min(n0 + a.W, a.max_len);
-  const Share share = share_of(end, a.splits);
-  if (split >= share.active) return;
-  const int rows = a.T * a.rep;
-  const int row0 = rb * kMT * 16;
+// 32 keys and their values, as a wave loads them, and as operands.
+template <typename T, CacheKind kKind, int kD>
+struct Tile : Shape<T, kKind, kD> {
+  using S = Shape<T, kKind, kD>;
+  using OV = typename Operand<T>::V;
+  static constexpr int kLoad = S::kSame || S::kPaired ? 16 : 8;
+  static constexpr int kLoads = S::kPaired ? S::kQK / 2 : S::kQK;
+  Raw<kLoad> k[2][kLoads];
+  Raw<S::kND * S::kBytes> v[8];
+  float kown[2];          // kFolded: the scales of the keys c of the two halves
+  f32x4 kscale[2], vscale[2];  // of the keys 4 g + r of the two halves
 
-  // the queries, as operands: 8 values of row c. Rows behind the last repeat
-  // it; no row reaches another's result, and they are not written.
-  OV q[kMT][kQK];
+  __device__ __forceinline__ void load_keys(const uint8_t* keys, const float* scales, int key0, int c, int g) {
+    const uint8_t* p = keys + (int64_t)key0 * S::kRowBytes + c * S::kRowBytes + g * kLoad;
 #pragma unroll
-  for (int mt = 0; mt < kMT; ++mt) {
-    const int row = min(row0 + mt * 16 + c, rows - 1);
-    const int t = row / a.rep, head = h * a.rep + row % a.rep;
-    const T* src = reinterpret_cast<const T*>(a.q) + b * a.qb + head * a.qh + t * a.qt;
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int ds = 0; ds < kQK; ++ds) {
-      const int d = kPaired ? (ds / 2) * 64 + g * 16 + (ds & 1) * 8 : ds * 32 + g * 8;
-      q[mt][ds] = *reinterpret_cast<const OV*>(src + d);
+      for (int i = 0; i < kLoads; ++i) k[t][i].load(p + t * 16 * S::kRowBytes + i * 64);
+      if constexpr (S::kFolded) kown[t] = scales[key0 + t * 16 + c];
+      if constexpr (S::kScaled) kscale[t] = *reinterpret_cast<const f32x4*>(scales + key0 + t * 16 + g * 4);
     }
   }
 
-  f32x4 o[kMT][kND];
-  float m[kMT], l[kMT];
+  __device__ __forceinline__ void load_values(const uint8_t* values, const float* scales, int key0, int c, int g) {
+    const uint8_t* p = values + (int64_t)key0 * S::kRowBytes + g * 4 * S::kRowBytes + c * S::kND * S::kBytes;
 #pragma unroll
-  for (int mt = 0; mt < kMT; ++mt) {
-    m[mt] = kNegInf;
-    l[mt] = 0.f;
+    for (int e = 0; e < 8; ++e) v[e].load(p + ((e >> 2) * 16 + (e & 3)) * S::kRowBytes);
+    if constexpr (!S::kSame) {
 #pragma unroll
-    for (int j = 0; j < kND; ++j) o[mt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 2; ++t) vscale[t] = *reinterpret_cast<const f32x4*>(scales + key0 + t * 16 + g * 4);
+    }
   }
-  constexpr unsigned kExp = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;  // of an infinity or NaN
-  bool odd = false;  // whether masked tiles have such values
-  int unit = -126;  // fp16, 8 bits: o is held in units of 2^unit (below)
 
-  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k) + (int64_t)bh * a.slots * kRowBytes;
-  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v) + (int64_t)bh * a.slots * kRowBytes;
-  const float* ks = kSame ? nullptr : a.k_scale + (int64_t)bh * a.slots;
-  const float* vs = kSame ? nullptr : a.v_scale + (int64_t)bh * a.slots;
-  const int first = split * share.steps * kStep + wave * kTile;
-  const int stop = min(end, (split + 1) * share.steps * kStep);
-
-  // A tile's keys are loaded while the tile before is exponentiated and
-  // multiplied with its values, its values while its own scores are made: the
-  // registers of one are free when the other's next loads start.
-  constexpr int kLoad = kSame || kPaired ? 16 : 8;
-  constexpr int kLoads = kPaired ? kQK / 2 : kQK;
-  Raw<kLoad> kraw[2][kLoads];
-  Raw<kND * kBytes> vraw[8];
-  f32x4 kscale[2], vscale[2];
-  const auto load_keys = [&](int key0) {
-    const uint8_t* kp = kbase + (int64_t)key0 * kRowBytes + c * kRowBytes + g * kLoad;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) kraw[t][i].load(kp + t * 16 * kRowBytes + i * 64);
-    if constexpr (!kSame) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) kscale[t] = *reinterpret_cast<const f32x4*>(ks + key0 + t * 16 + g * 4);
+  __device__ __forceinline__ OV key(int t, int ds) const {
+    if constexpr (S::kSame) {
+      return __builtin_bit_cast(OV, k[t][ds]);
+    } else {
+      const auto& raw = k[t][S::kPaired ? ds / 2 : ds];
+      const int w0 = S::kPaired ? (ds & 1) * 2 : 0;
+      const float scale = S::kFolded ? kown[t] : 1.f;
+      return __builtin_bit_cast(
+          OV, uint4v{decode2<T, kKind, false>(raw.w[w0], scale), decode2<T, kKind, true>(raw.w[w0], scale),
+                     decode2<T, kKind, false>(raw.w[w0 + 1], scale), decode2<T, kKind, true>(raw.w[w0 + 1], scale)});
     }
-  };
-  const auto load_values = [&](int key0) {
-    const uint8_t* vp = vbase + (int64_t)key0 * kRowBytes + g * 4 * kRowBytes + c * kND * kBytes;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) vraw[e].load(vp + ((e >> 2) * 16 + (e & 3)) * kRowBytes);
-    if constexpr (!kSame) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) vscale[t] = *reinterpret_cast<const f32x4*>(vs + key0 + t * 16 + g * 4);
-    }
-  };
-  // No load is conditional: a wave without keys, or without more, reads its
-  // last tile or the sequence's first once more, from a cache. Registers that
-  // a branch may leave unwritten were given away by the compiler while they
-  // were in use.
-  const int safe = first < stop ? first : 0;
-  load_keys(safe);
-  load_values(safe);
-  for (int key0 = first; key0 < stop; key0 += kStep) {
-    const int next = key0 + kStep < stop ? key0 + kStep : key0;
+  }
 
-    // scores
-    f32x4 s[kMT][2];
+  // Operands j and j + 1: the j-th and next values of the lane's eight keys.
+  __device__ __forceinline__ void value2(int j, OV& x, OV& y) const {
+    uint4v lo, hi;
 #pragma unroll
-    for (int mt = 0; mt < kMT; ++mt) s[mt][0] = s[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ds = 0; ds < kQK; ++ds) {
-      OV k[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if constexpr (kSame) {
-          k[t] = __builtin_bit_cast(OV, kraw[t][ds]);
+    for (int e = 0; e < 8; e += 2) {
+      if constexpr (S::kScaled) {
+        lo[e / 2] = decode_bytes<T, kKind>(v[e].w[j / 4], v[e + 1].w[j / 4], j & 3);
+        hi[e / 2] = decode_bytes<T, kKind>(v[e].w[j / 4], v[e + 1].w[j / 4], (j & 3) + 1);
+      } else {
+        unsigned a, b;
+        if constexpr (S::kSame) {
+          a = v[e].w[j / 2];
+          b = v[e + 1].w[j / 2];
+        } else if (j & 2) {
+          a = decode2<T, kKind, true>(v[e].w[j / 4], vscale[e >> 2][e & 3]);
+          b = decode2<T, kKind, true>(v[e + 1].w[j / 4], vscale[e >> 2][(e & 3) + 1]);
         } else {
-          const auto& raw = kraw[t][kPaired ? ds / 2 : ds];
-          const int w0 = kPaired ? (ds & 1) * 2 : 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) k[t][i] = (T)decode<kKind>(raw.w[w0 + i / 4], i & 3);
+          a = decode2<T, kKind, false>(v[e].w[j / 4], vscale[e >> 2][e & 3]);
+          b = decode2<T, kKind, false>(v[e + 1].w[j / 4], vscale[e >> 2][(e & 3) + 1]);
         }
-      }
-#pragma unroll
-      for (int mt = 0; mt < kMT; ++mt)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) s[mt][t] = Op::mfma(k[t], q[mt][ds], s[mt][t]);
-    }
-    float ksc[8], vsc[8];
-    if constexpr (!kSame) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        ksc[e] = kscale[e >> 2][e & 3] * a.scale_log2;
-        vsc[e] = vscale[e >> 2][e & 3];
+        lo[e / 2] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        hi[e / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
       }
     }
-    load_keys(next);
+    x = __builtin_bit_cast(OV, lo);
+    y = __builtin_bit_cast(OV, hi);
+  }
 
-    const bool masked = key0 + kTile > n0;  // the tile has slots that some rows do not see
-    float p[kMT][8];
-    bool grew = false;
-    float keep[kMT];
+  // A probability of zero does not hide an infinite or NaN value. In a tile
+  // with slots that some rows do not see, slots behind the new tokens (which
+  // hold anything) are cleared; of the others, values that are not finite are
+  // left out and added at the end, to the rows that see them alone. Says
+  // whether there are any.
+  __device__ __forceinline__ bool clear(int key0, int end, int g) {
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = key0 + (e >> 2) * 16 + g * 4 + (e & 3) < end;
+      if constexpr (S::kSame) {
+#pragma unroll
+        for (int w = 0; w < Raw<S::kND * S::kBytes>::kWords; ++w) {
+          unsigned& x = v[e].w[w];
+          const unsigned low = (x & S::kExp) == S::kExp ? 0xFFFFu : 0u;
+          const unsigned high = ((x >> 16) & S::kExp) == S::kExp ? 0xFFFF0000u : 0u;
+          odd |= in & ((low | high) != 0);
+          x = in ? x & ~(low | high) : 0u;
+        }
+      } else {  // codes are finite, their scale may not be
+        const float x = vscale[e >> 2][e & 3];
+        const bool finite = x < __builtin_inff();
+        odd |= in & !finite;
+        vscale[e >> 2][e & 3] = in & finite ? x : 0.f;
+      }
+    }
+    return odd;
+  }
+};
+
+// A wave's rows: queries, running maximum and sum of the softmax, and sums of
+// values. Row c of tile mt belongs to the four lanes c + 16 g.
+template <typename T, CacheKind kKind, int kD, int kMT>
+struct Rows : Shape<T, kKind, kD> {
+  using S = Shape<T, kKind, kD>;
+  using OV = typename Operand<T>::V;
+  // 8-bit values times probabilities would be lost below fp16's range
+  static constexpr bool kUnits = S::kScaled && __is_same(T, _Float16);
+  OV q[kMT][S::kQK];
+  f32x4 o[kMT][S::kND];
+  float m[kMT], l[kMT];
+  float scale;  // of the scores where the keys' are none, not negative
+  int unit;     // o is held in units of 2^unit (kUnits)
+
+  __device__ __forceinline__ void start(const AttendArgs& a, const Work& w, int row0, int c, int g) {
+    // Rows behind the last repeat it; no row reaches another's result, and
+    // they are not written.
+    const int rows = a.T * a.rep;
+    unit = -126;
+    // The largest score is the largest product, so that only one a row has to
+    // be scaled before the exponentials. A negative scale turns the queries.
+    scale = fmaxf(fabsf(a.scale_log2), 0x1p-126f);  // not zero: times minus infinity that is NaN
+    const unsigned turn = !S::kScaled && a.scale_log2 < 0.f ? 0x80008000u : 0u;
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt) {
-      const int t_row = (row0 + mt * 16 + c) / a.rep;
+      const int row = min(row0 + mt * 16 + c, rows - 1);
+      const int t = row / a.rep, head = w.h * a.rep + row % a.rep;
+      const T* src = reinterpret_cast<const T*>(a.q) + w.b * a.qb + head * a.qh + t * a.qt;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[mt][e] = s[mt][e >> 2][e & 3] * (kSame ? a.scale_log2 : ksc[e]);
-      if (masked) {
+      for (int ds = 0; ds < S::kQK; ++ds) {
+        const int d = S::kPaired ? (ds / 2) * 64 + g * 16 + (ds & 1) * 8 : ds * 32 + g * 8;
+        q[mt][ds] = __builtin_bit_cast(OV, *reinterpret_cast<const uint4v*>(src + d) ^ turn);
+      }
+      m[mt] = kNothing;
+      l[mt] = 0.f;
+#pragma unroll
+      for (int j = 0; j < S::kND; ++j) o[mt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // Scores of the 32 keys from key0 on to probabilities, as operands; o and l
+  // follow the maximum.
+  __device__ __forceinline__ void soften(const AttendArgs& a, const Work& w, const f32x4 (&s)[kMT][2],
+                                         const f32x4* kscale, const f32x4* vscale, int key0, int row0, int c, int g,
+                                         OV (&pv)[kMT]) {
+    const bool masked = key0 + kTile > w.n0;  // the tile has slots that some rows do not see
+    bool grew = false;
+    float p[kMT][8], keep[kMT];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float ksc = S::kScaled ? kscale[e >> 2][e & 3] * a.scale_log2 : 1.f;
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt) p[mt][e] = S::kScaled ? s[mt][e >> 2][e & 3] * ksc : s[mt][e >> 2][e & 3];
+    }
+    if (masked) {
+      // Selects, no branches: an array element written under a lane's own
+      // condition was lost by the compiler.
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt) {
+        const int t_row = (row0 + mt * 16 + c) / a.rep;
         // all of a lane's mask values are read at once, from inside the mask
         const bool chain = a.mask == nullptr;
-        const uint8_t* bits = a.mask + b * a.mb + min(t_row, a.T - 1) * a.mt;
+        const uint8_t* bits = a.mask + w.b * a.mb + min(t_row, a.T - 1) * a.mt;
         uint8_t bit[8] = {};
         if (!chain && a.W > 0) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) bit[e] = bits[min(max(key0 + (e >> 2) * 16 + g * 4 + (e & 3) - n0, 0), a.W - 1)];
+          for (int e = 0; e < 8; ++e)
+            bit[e] = bits[min(max(key0 + (e >> 2) * 16 + g * 4 + (e & 3) - w.n0, 0), a.W - 1)];
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int key = key0 + (e >> 2) * 16 + g * 4 + (e & 3);
-          // selects, no branches: an array element written under a lane's own
-          // condition was lost by the compiler
-          const bool sees = (key < n0) | ((key < end) & (chain ? key - n0 <= t_row : bit[e] != 0));
+          const bool sees = (key < w.n0) | ((key < w.end) & (chain ? key - w.n0 <= t_row : bit[e] != 0));
           p[mt][e] = sees ? p[mt][e] : kNegInf;
         }
       }
-      float top = p[mt][0];
+    }
 #pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, p[mt][e]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+    for (int mt = 0; mt < kMT; ++mt) {
+      float top = fmaxf(p[mt][0], p[mt][1]);
+#pragma unroll
+      for (int e = 2; e < 8; ++e) top = fmaxf(top, p[mt][e]);
+      top = max_over_groups(top);
+      if constexpr (!S::kScaled) top *= scale;
       const float m_new = fmaxf(m[mt], top);
-      const float base = m_new == kNegInf ? 0.f : m_new;  // nothing seen so far
-      keep[mt] = __builtin_amdgcn_exp2f(m[mt] - base);
+      keep[mt] = __builtin_amdgcn_exp2f(m[mt] - m_new);
       grew |= m_new > m[mt];
       m[mt] = m_new;
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[mt][e] = __builtin_amdgcn_exp2f(p[mt][e] - base);
+        p[mt][e] = __builtin_amdgcn_exp2f(S::kScaled ? p[mt][e] - m_new : __builtin_fmaf(p[mt][e], scale, -m_new));
         sum += p[mt][e];
       }
       l[mt] = l[mt] * keep[mt] + sum;
     }
 
-    if constexpr (!kSame) {
-      if (masked) {  // slots behind the new tokens hold anything
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          vsc[e] = key0 + (e >> 2) * 16 + g * 4 + (e & 3) < end ? vsc[e] : 0.f;
-      }
-    }
     float unit_scale = 1.f;
-    if constexpr (!kSame && __is_same(T, _Float16)) {
-      // Probabilities times the values' scales would be lost below fp16's
-      // range. They are held relative to the power of two of the largest
+    if constexpr (kUnits) {
+      // Probabilities are held relative to the power of two of the largest
       // scale so far, which is the same for all rows.
       float most = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, vsc[e]);
-#pragma unroll
-      for (int x = 16; x < 64; x <<= 1) most = fmaxf(most, __shfl_xor(most, x));
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, vscale[e >> 2][e & 3]);
+      most = max_over_groups(most);
       const int wanted = min(max(unit, (int)(__float_as_uint(most) >> 23) - 126), 120);
-      if (wanted > unit) {
-        grew = true;
-        const float less = __builtin_ldexpf(1.f, max(unit - wanted, -126));
+      const float less = __builtin_ldexpf(1.f, max(unit - wanted, -126));
+      grew |= wanted > unit;
 #pragma unroll
-        for (int mt = 0; mt < kMT; ++mt) keep[mt] *= less;
-        unit = wanted;
-      }
+      for (int mt = 0; mt < kMT; ++mt) keep[mt] *= less;
+      unit = wanted;
       unit_scale = __builtin_ldexpf(1.f, -unit);
     }
     if (__any(grew)) {
 #pragma unroll
       for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
-        for (int j = 0; j < kND; ++j) o[mt][j] *= keep[mt];
+        for (int j = 0; j < S::kND; ++j) o[mt][j] *= keep[mt];
     }
 
     // Probabilities are rounded to the type of the product's operands: half a
     // step of it for each, without a common sign.
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt) {
+      uint4v x;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        if constexpr (S::kScaled)
+          x[e / 2] = pack2<T>(p[mt][e] * (vscale[e >> 2][e & 3] * unit_scale),
+                              p[mt][e + 1] * (vscale[e >> 2][(e & 3) + 1] * unit_scale));
+        else
+          x[e / 2] = pack2<T>(p[mt][e], p[mt][e + 1]);
+      }
+      pv[mt] = __builtin_bit_cast(OV, x);
+    }
+  }
+
+  // The sums of a row over its four lanes; o in units of 1.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt) {
+      l[mt] = sum_over_groups(l[mt]);
+      if constexpr (kUnits) {
+        const float one = __builtin_ldexpf(1.f, unit);
+#pragma unroll
+        for (int j = 0; j < S::kND; ++j) o[mt][j] *= one;
+      }
+    }
+  }
+};
+
+// The infinite and NaN values (8 bits: the values of such scales) that the
+// masked tiles left out, of the workgroup's slots that row t sees, added to its
+// sums of N dimensions from d on.
+template <typename T, int N>
+__device__ void add_odd_row(const AttendArgs& a, const Work& w, int t, const uint8_t* values, const float* scales, int d,
+                            float* y) {
+  for (int j = max(w.from, w.n0 / kTile * kTile); j < w.stop; ++j) {
+    if (j >= w.n0 && !(a.mask ? a.mask[w.b * a.mb + t * a.mt + (j - w.n0)] != 0 : j - w.n0 <= t)) continue;
+    for (int i = 0; i < N; ++i) {
+      const float v = scales ? scales[j] : (float)reinterpret_cast<const T*>(values)[(int64_t)j * a.D + d + i];
+      if (!__builtin_isfinite(v)) y[i] += scales ? __builtin_nanf("") : v;
+    }
+  }
+}
+
+// N dimensions of a row from d on, as the result or as a split's part of it.
+template <typename T, int N>
+__device__ __forceinline__ void write_row(const AttendArgs& a, const Work& w, int row, int d, const float* y, float top,
+                                          float sum) {
+  if (a.splits == 1) {
+    const int t = row / a.rep, head = w.h * a.rep + row % a.rep;
+    const float inverse = 1.f / sum;
+    const float none = sum == 0.f ? empty_row(a, w.b, t, w.n0) : 0.f;
+    struct alignas(N * 2 < 16 ? N * 2 : 16) { T v[N]; } out;
+#pragma unroll
+    for (int j = 0; j < N; ++j) out.v[j] = (T)(sum == 0.f ? none : y[j] * inverse);
+    *reinterpret_cast<decltype(out)*>(reinterpret_cast<T*>(a.out) + w.b * a.ob + head * a.oh + t * a.ot + d) = out;
+  } else {
+    const int64_t at = ((int64_t)w.bh * a.T * a.rep + row) * a.splits + w.split;
+    struct alignas(N * 4 < 16 ? N * 4 : 16) { float v[N]; } out;
+#pragma unroll
+    for (int j = 0; j < N; ++j) out.v[j] = y[j];
+    *reinterpret_cast<decltype(out)*>(a.part_o + at * a.D + d) = out;
+    if (d == 0) {
+      a.part_ml[at * 2] = top;
+      a.part_ml[at * 2 + 1] = sum;
+    }
+  }
+}
+
+// The four waves of a workgroup take tiles of keys in turn, all for the same
+// 16 kMT rows, and join in the end.
+template <typename T, CacheKind kKind, int kD, int kMT>
+__global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(AttendArgs a) {
+  using S = Shape<T, kKind, kD>;
+  using OV = typename Operand<T>::V;
+  constexpr int kND = S::kND;
+  __shared__ float red[kWaves][4][kND][64];
+  __shared__ float red_m[kWaves][kMT][16], red_l[kWaves][kMT][16];
+  __shared__ int red_odd;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const Work w = work_of(a);
+  if (!w.any) return;
+  const int row0 = w.rb * kMT * 16;
+  const uint8_t* keys = reinterpret_cast<const uint8_t*>(a.k) + (int64_t)w.bh * a.slots * S::kRowBytes;
+  const uint8_t* values = reinterpret_cast<const uint8_t*>(a.v) + (int64_t)w.bh * a.slots * S::kRowBytes;
+  const float* ks = S::kSame ? nullptr : a.k_scale + (int64_t)w.bh * a.slots;
+  const float* vs = S::kSame ? nullptr : a.v_scale + (int64_t)w.bh * a.slots;
+  bool odd = false;  // whether masked tiles have values that are not finite
+
+  // A tile's keys are loaded while the tile before is exponentiated and
+  // multiplied with its values, its values while its own scores are made: the
+  // registers of one are free when the other's next loads start. No load is
+  // conditional: a wave without keys, or without more, reads its last tile or
+  // the sequence's first once more, from a cache. Registers that a branch may
+  // leave unwritten were given away by the compiler while they were in use.
+  Tile<T, kKind, kD> tile;
+  const int first = w.from + wave * kTile;
+  const int safe = first < w.stop ? first : 0;
+  tile.load_keys(keys, ks, safe, c, g);
+  tile.load_values(values, vs, safe, c, g);
+  Rows<T, kKind, kD, kMT> rows;
+  rows.start(a, w, row0, c, g);
+  for (int key0 = first; key0 < w.stop; key0 += kStep) {
+    const int next = key0 + kStep < w.stop ? key0 + kStep : key0;
+    f32x4 s[kMT][2];
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt) s[mt][0] = s[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ds = 0; ds < S::kQK; ++ds) {
+      const OV k0 = tile.key(0, ds), k1 = tile.key(1, ds);
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt) {
+        s[mt][0] = Operand<T>::mfma(k0, rows.q[mt][ds], s[mt][0]);
+        s[mt][1] = Operand<T>::mfma(k1, rows.q[mt][ds], s[mt][1]);
+      }
+    }
+    const f32x4 kscale[2] = {tile.kscale[0], tile.kscale[1]};
+    tile.load_keys(keys, ks, next, c, g);
+    if (key0 + kTile > w.n0) odd |= tile.clear(key0, w.end, g);
     OV pv[kMT];
+    rows.soften(a, w, s, kscale, tile.vscale, key0, row0, c, g, pv);
 #pragma unroll
-    for (int mt = 0; mt < kMT; ++mt)
+    for (int j = 0; j < kND; j += 2) {
+      OV v0, v1;
+      tile.value2(j, v0, v1);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float x = p[mt][e];
-        if constexpr (!kSame) {
-          x *= vsc[e] * unit_scale;
-          // the scale of a token that the row does not see may be anything
-          x = masked & (p[mt][e] == 0.f) ? 0.f : x;
-        }
-        pv[mt][e] = (T)x;
-      }
-
-    if constexpr (kSame) {
-      if (masked) {
-        // A probability of zero does not hide an infinite or NaN value. Slots
-        // behind the new tokens are cleared; of the others, those values that
-        // are not finite are left out here and added at the end, to the rows
-        // that see them alone.
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool in = key0 + (e >> 2) * 16 + g * 4 + (e & 3) < end;
-#pragma unroll
-          for (int w = 0; w < Raw<kND * kBytes>::kWords; ++w) {
-            unsigned& x = vraw[e].w[w];
-            const unsigned low = (x & kExp) == kExp ? 0xFFFFu : 0u;
-            const unsigned high = ((x >> 16) & kExp) == kExp ? 0xFFFF0000u : 0u;
-            odd |= in & ((low | high) != 0);
-            x = in ? x & ~(low | high) : 0u;
-          }
-        }
+      for (int mt = 0; mt < kMT; ++mt) {
+        rows.o[mt][j] = Operand<T>::mfma(v0, pv[mt], rows.o[mt][j]);
+        rows.o[mt][j + 1] = Operand<T>::mfma(v1, pv[mt], rows.o[mt][j + 1]);
       }
     }
-
-#pragma unroll
-    for (int j = 0; j < kND; ++j) {
-      OV v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (kSame) v[e] = vraw[e].template as16<T>(j);
-        else v[e] = (T)decode<kKind>(vraw[e].w[j / 4], j & 3);
-      }
-#pragma unroll
-      for (int mt = 0; mt < kMT; ++mt) o[mt][j] = Op::mfma(v, pv[mt], o[mt][j]);
-    }
-    load_values(next);
+    tile.load_values(values, vs, next, c, g);
   }
 
   // the four waves' parts of a row, joined
+  rows.finish();
   if (threadIdx.x == 0) red_odd = 0;
   __syncthreads();
-  if (kSame && odd) red_odd = 1;
+  if (odd) red_odd = 1;
+  if (g == 0) {
 #pragma unroll
-  for (int mt = 0; mt < kMT; ++mt) {
-    l[mt] += __shfl_xor(l[mt], 16);
-    l[mt] += __shfl_xor(l[mt], 32);
-    if (g == 0) {
-      red_m[wave][mt][c] = m[mt];
-      red_l[wave][mt][c] = l[mt];
+    for (int mt = 0; mt < kMT; ++mt) {
+      red_m[wave][mt][c] = rows.m[mt];
+      red_l[wave][mt][c] = rows.l[mt];
     }
   }
   __syncthreads();
 #pragma unroll
   for (int mt = 0; mt < kMT; ++mt) {
-    float top = kNegInf, sum = 0.f;
+    float top = kNothing, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red_m[w][mt][c]);
-    const float base = top == kNegInf ? 0.f : top;
+    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, red_m[i][mt][c]);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += red_l[w][mt][c] * __builtin_amdgcn_exp2f(red_m[w][mt][c] - base);
-    float mine = __builtin_amdgcn_exp2f(m[mt] - base);
-    if constexpr (!kSame && __is_same(T, _Float16)) mine *= __builtin_ldexpf(1.f, unit);
+    for (int i = 0; i < kWaves; ++i) sum += red_l[i][mt][c] * __builtin_amdgcn_exp2f(red_m[i][mt][c] - top);
+    const float mine = __builtin_amdgcn_exp2f(rows.m[mt] - top);
 #pragma unroll
     for (int j = 0; j < kND; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) red[wave][r][j][lane] = o[mt][j][r] * mine;
+      for (int r = 0; r < 4; ++r) red[wave][r][j][lane] = rows.o[mt][j][r] * mine;
     __syncthreads();
-    // wave w sums the elements r = w: neighbours of row c from (4 g + w) D / 16 on
+    // wave i sums the elements r = i: neighbours of row c from (4 g + i) D / 16 on
     const int row = row0 + mt * 16 + c;
     float y[kND];
 #pragma unroll
     for (int j = 0; j < kND; ++j) {
       y[j] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) y[j] += red[w][wave][j][lane];
+      for (int i = 0; i < kWaves; ++i) y[j] += red[i][wave][j][lane];
     }
     __syncthreads();
-    if (row < rows) {
+    if (row < a.T * a.rep) {
       const int d = (g * 4 + wave) * kND;
-      if (kSame && red_odd) add_odd_row<T, kND>(a, b, row / a.rep, n0, first - wave * kTile, stop, vbase, d, y);
-      if (a.splits == 1) {
-        const int t = row / a.rep, head = h * a.rep + row % a.rep;
-        const float inverse = 1.f / sum;
-        T* dst = reinterpret_cast<T*>(a.out) + b * a.ob + head * a.oh + t * a.ot + d;
-        const float none = sum == 0.f ? empty_row(a, b, t, n0) : 0.f;
-        struct alignas(kND * 2 < 16 ? kND * 2 : 16) { T v[kND]; } out;
-#pragma unroll
-        for (int j = 0; j < kND; ++j) out.v[j] = (T)(sum == 0.f ? none : y[j] * inverse);
-        *reinterpret_cast<decltype(out)*>(dst) = out;
-      } else {
-        const int64_t at = ((int64_t)bh * rows + row) * a.splits + split;
-        struct alignas(kND * 4 < 16 ? kND * 4 : 16) { float v[kND]; } out;
-#pragma unroll
-        for (int j = 0; j < kND; ++j) out.v[j] = y[j];
-        *reinterpret_cast<decltype(out)*>(a.part_o + at * kD + d) = out;
-        if (d == 0) {
-          a.part_ml[at * 2] = top;
-          a.part_ml[at * 2 + 1] = sum;
-        }
-      }
+      if (red_odd) add_odd_row<T, kND>(a, w, row / a.rep, values, vs, d, y);
+      write_row<T, kND>(a, w, row, d, y, top, sum);
     }
   }
 }
 
-// The splits of a row, joined: a workgroup a row. Its threads take four
+// The splits of a row, joined, where they are few: D / 4 lanes a row, each of
+// four dimensions.
+template <typename T, int kD>
+__global__ void __launch_bounds__(256) attend_join_few_kernel(AttendArgs a) {
+  constexpr int kLanes = kD / 4;
+  const int rows = a.T * a.rep;
+  const int lane = threadIdx.x % kLanes;
+  const int64_t at_row = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (at_row >= (int64_t)a.B * a.Hkv * rows) return;
+  const int bh = (int)(at_row / rows), row = (int)(at_row - (int64_t)bh * rows);
+  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const int n0 = clamped_length(a, b);
+  const int active = share_of(min(n0 + a.W, a.max_len), a).active;
+  const float* ml = a.part_ml + at_row * a.splits * 2;
+  const float* part = a.part_o + at_row * a.splits * kD + lane * 4;
+  float m[kFewSplits], l[kFewSplits];
+  f32x4 o[kFewSplits];
+  float top = kNothing;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {  // splits behind the last repeat it, with no weight
+    const int at = min(s, active - 1);
+    m[s] = ml[at * 2];
+    l[s] = ml[at * 2 + 1];
+    o[s] = *reinterpret_cast<const f32x4*>(part + at * kD);
+    top = fmaxf(top, m[s]);
+  }
+  float sum = 0.f;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    const float weight = __builtin_amdgcn_exp2f(m[s] - top);
+    const bool is = s < active;
+    sum += is ? l[s] * weight : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] += is ? o[s][i] * weight : 0.f;
+  }
+  const int t = row / a.rep, head = h * a.rep + row % a.rep;
+  const float none = sum == 0.f ? empty_row(a, b, t, n0) : 0.f, inverse = 1.f / sum;
+  struct alignas(8) { T v[4]; } out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out.v[i] = (T)(sum == 0.f ? none : y[i] * inverse);
+  *reinterpret_cast<decltype(out)*>(reinterpret_cast<T*>(a.out) + b * a.ob + head * a.oh + t * a.ot + lane * 4) = out;
+}
+
+// Where they are many: a workgroup a row. Its threads take four
 // dimensions each and share the splits out, so that few rows of many splits
 // (one long sequence) still have many reads under way.
 template <typename T, int kD>
@@ -495,14 +667,14 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   const int bh = blockIdx.x / rows, row = blockIdx.x - bh * rows;
   const int b = bh / a.Hkv, h = bh - b * a.Hkv;
   const int n0 = clamped_length(a, b);
-  const int active = share_of(min(n0 + a.W, a.max_len), a.splits).active;
+  const int active = share_of(min(n0 + a.W, a.max_len), a).active;
   const int64_t at = (int64_t)blockIdx.x * a.splits;
 
-  float m[kMaxSplits / 256], l[kMaxSplits / 256], top = kNegInf;
+  float m[kMaxSplits / 256], l[kMaxSplits / 256], top = kNothing;
 #pragma unroll
   for (int i = 0; i < kMaxSplits / 256; ++i) {
     const int s = tid + i * 256;
-    m[i] = kNegInf;
+    m[i] = kNothing;
     l[i] = 0.f;
     if (s < active) {
       m[i] = a.part_ml[(at + s) * 2];
@@ -515,11 +687,10 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   if ((tid & 63) == 0) red_m[tid >> 6] = top;
   __syncthreads();
   top = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
-  const float base = top == kNegInf ? 0.f : top;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kMaxSplits / 256; ++i) {
-    const float w = __builtin_amdgcn_exp2f(m[i] - base);
+    const float w = __builtin_amdgcn_exp2f(m[i] - top);
     weight[tid + i * 256] = w;
     sum += l[i] * w;
   }
@@ -550,15 +721,13 @@ hipError_t attend_by_rows(const AttendArgs& a, hipStream_t stream) {
   const int64_t parts = (int64_t)a.splits * a.Hkv * a.B;
   const int64_t blocks = a.row_blocks == 1 ? parts : (parts + 7) / 8 * 8 * a.row_blocks;
   const dim3 grid((unsigned)blocks), block(256);
-  switch (attend_row_tiles(a.T * a.rep, kD)) {
-    case 1: hipLaunchKernelGGL((attend_kernel<T, kKind, kD, 1>), grid, block, 0, stream, a); break;
-    case 2: hipLaunchKernelGGL((attend_kernel<T, kKind, kD, 2>), grid, block, 0, stream, a); break;
-    default:
-      if constexpr (kD <= 128) hipLaunchKernelGGL((attend_kernel<T, kKind, kD, 4>), grid, block, 0, stream, a);
-      break;
-  }
-  if (a.splits > 1)
-    hipLaunchKernelGGL((attend_join_kernel<T, kD>), dim3((unsigned)(a.B * a.Hkv * a.T * a.rep)), block, 0, stream, a);
+  if (a.T * a.rep <= 16) hipLaunchKernelGGL((attend_kernel<T, kKind, kD, 1>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((attend_kernel<T, kKind, kD, 2>), grid, block, 0, stream, a);
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.T * a.rep, per = 256 / (kD / 4);
+  if (a.splits > kFewSplits)
+    hipLaunchKernelGGL((attend_join_kernel<T, kD>), dim3((unsigned)rows), block, 0, stream, a);
+  else if (a.splits > 1)
+    hipLaunchKernelGGL((attend_join_few_kernel<T, kD>), dim3((unsigned)((rows + per - 1) / per)), block, 0, stream, a);
   return hipGetLastError();
 }
 
@@ -583,22 +752,30 @@ hipError_t attend_by_kind(const AttendArgs& a, CacheKind kind, hipStream_t strea
 
 }  // namespace
 
-// Tiles of 16 rows a workgroup holds. More rows share one reading of the keys;
-// at D = 256 four tiles of accumulators would not fit the registers.
-int attend_row_tiles(int rows, int D) {
-  if (rows <= 16) return 1;
-  return rows <= 32 || D == 256 ? 2 : 4;
-}
-
-// Parts that a sequence's keys are split into: enough workgroups for two on
-// each of the 256 CUs, and none with less than one step of keys. The host does
-// not know the lengths, so the cache's size stands for them; a shorter
-// sequence is shared out over the same number, as far as its steps go.
-int attend_splits(const AttendArgs& a) {
+// Row blocks: 32 rows leave two waves a SIMD room. 64 (one wave) took 68 us
+// where these take 41 (8 sequences, 8 heads, 108 rows, 4000 e4m3 keys); a
+// workgroup that shares its decoded keys among 128 rows, in LDS, took 43.
+//
+// Splits of the keys: the host does not know the lengths, so the cache's size
+// stands for them; a shorter sequence is shared out over the same number, as
+// far as its steps go.
+//  * Up to 4 steps there is one, and no second launch (300 keys: 6.7 to 8.2 us
+//    with one, 7.5 to 8.1 with three; the host issues one in 7 us, two in 10).
+//  * Else one workgroup a CU: 16000 keys of 8 heads take 17.5 (bf16) and 13.0
+//    us (int8) with 32 splits, 19.4 and 14.4 with 64.
+//  * Two, where the parts stay long: then the second hides what the first
+//    waits for, and sequences of unlike length even out (130000 int8 keys of 8
+//    heads: 54.6 us with 32, 47.5 with 64; 32 sequences of up to 16000: 199 and
+//    156 us with one and two).
+void plan_attend(AttendArgs& a) {
+  const int rows = a.T * a.rep, per = rows <= 16 ? 16 : 32;
+  a.row_blocks = (rows + per - 1) / per;
+  a.splits = 1;
+  if (a.max_len <= 4 * kStep) return;
   const int64_t groups = (int64_t)a.B * a.Hkv * a.row_blocks;
-  const int64_t wanted = (kMaxSplits + groups - 1) / groups;
-  const int64_t most = (a.max_len + kStep - 1) / kStep;
-  return (int)std::max<int64_t>(1, std::min(wanted, most));
+  int64_t splits = (256 + groups - 1) / groups;
+  if (a.max_len / splits >= 2048) splits = (512 + groups - 1) / groups;
+  a.splits = (int)std::min<int64_t>(splits, (a.max_len + kStep - 1) / kStep);
 }
 
 hipError_t launch_attend(const AttendArgs& a, ServingType type, CacheKind kind, hipStream_t stream) {

@@ -55,7 +55,8 @@ struct AttendArgs {
   const uint8_t* mask;         // [B, T, W] truth values, or null: the causal chain
   float *part_o, *part_ml;     // [B * Hkv, rows, splits, D] and [.., 2]
   int64_t qb, qh, qt, ob, oh, ot, mb, mt;
-  int B, Hkv, rep, T, W, D, slots, max_len, splits, row_blocks;
+  int B, Hkv, rep, T, W, D, slots, max_len;
+  int splits, row_blocks;      // set by plan_attend
   float scale_log2;            // the softmax scale times log2(e)
 };
 
@@ -79,7 +80,6 @@ hipError_t launch_rotary(RotaryArgs a, ServingType type, int V, bool interleaved
 hipError_t launch_cache_append(const CacheArgs& a, ServingType type, CacheKind kind, hipStream_t stream);
 hipError_t launch_cache_read(const CacheArgs& a, ServingType type, CacheKind kind, ServingType out, hipStream_t stream);
 hipError_t launch_cache_keep(const CacheArgs& a, const int64_t* path, int row_bytes, hipStream_t stream);
-int attend_row_tiles(int rows, int D);
-int attend_splits(const AttendArgs& a);
+void plan_attend(AttendArgs& a);
 hipError_t launch_attend(const AttendArgs& a, ServingType type, CacheKind kind, hipStream_t stream);
 hipError_t launch_verify(const VerifyArgs& a, ServingType type, hipStream_t stream);

@@ -391,9 +391,7 @@ at::Tensor kv_cache_attend(at::Tensor q, at::Tensor cache_k, at::Tensor cache_v,
   a.oh = out.stride(1);
   a.ot = out.stride(2);
   const int rows = (int)(T * a.rep);
-  const int per_block = 16 * attend_row_tiles(rows, c.D);
-  a.row_blocks = (rows + per_block - 1) / per_block;
-  a.splits = attend_splits(a);
+  plan_attend(a);
   TORCH_CHECK((int64_t)a.splits * c.H * c.B * a.row_blocks < kMaxInt - 8 * (int64_t)a.row_blocks, who, ": too many workgroups");
   at::Tensor part;
   if (a.splits > 1) {

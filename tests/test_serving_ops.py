@@ -1052,3 +1052,38 @@ def test_cache_without_slots_gives_zeros(device):
     assert not cache_attention(q, cache, mask=mask).any()
     with pytest.raises(RuntimeError):
         cache_attention(q, cache)
+
+
+@gpu
+@pytest.mark.parametrize("quant", [None, "int8"])
+@pytest.mark.parametrize("T", [3, 50])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30])
+def test_cache_attention_scales(quant, T, scale):
+    cache = filled_cache(2, 1, 200, 64, [0, 100], T, BF16, quant, "cuda")
+    q = randn(2, 2, T, 64, seed=73, dtype=BF16, device="cuda")
+    check_attention(cache_attention(q, cache, scale=scale), q, cache, None, scale)
+
+
+@gpu
+@pytest.mark.parametrize("quant", [None, "int8", "fp8"])
+@pytest.mark.parametrize("T", [5, 20, 70])
+def test_cache_attention_odd_tokens_reach_those_that_see_them(quant, T):
+    """A token with NaN among the new ones and one before them, for few and many rows, with splits."""
+    cache = filled_cache(1, 1, 700, 64, [600], T, BF16, quant, "cuda")
+    k, v = randn(1, 1, T, 64, seed=74, dtype=BF16, device="cuda"), randn(1, 1, T, 64, seed=75, dtype=BF16, device="cuda")
+    v[0, 0, 3, 9] = math.nan
+    cache.append(k, v)
+    q = randn(1, 2, T, 64, seed=76, dtype=BF16, device="cuda")
+    mask = (torch.rand(T, T, generator=torch.Generator().manual_seed(77)) < 0.5).cuda()
+    out = cache_attention(q, cache, mask=mask)
+    check_attention(out, q, cache, mask)
+    assert torch.equal(torch.isnan(out[0, 0, :, 9]), mask[:, 3]) and torch.isfinite(out[0, :, ~mask[:, 3]]).all()
+    # among those that stand: in a tile that all see, and in the last one before the new tokens
+    for slot in (100, 599):
+        cache.lengths.fill_(slot)
+        cache.append(k[:, :, 3:4], v[:, :, 3:4])
+        cache.lengths.fill_(600)
+        assert torch.isnan(cache_attention(q, cache, mask=mask)[..., 9]).all()
+        cache.lengths.fill_(slot)
+        cache.append(k[:, :, 2:3], v[:, :, 2:3])
+        cache.lengths.fill_(600)
