@@ -127,8 +127,8 @@ std::tuple<at::Tensor, OptTensor> rotate(at::Tensor q, OptTensor k, at::Tensor c
   a.Hq = (int)q.size(1);
   a.Hk = k.has_value() ? (int)k->size(1) : 0;
   if (a.tokens == 0 || a.Hq + a.Hk == 0 || D == 0) return {yq, yk};
-  // a token has at most max(64, D) threads of work, or all tokens have few
-  TORCH_CHECK(a.tokens < 256 * kMaxInt / std::max<int64_t>(64, D), who, ": too many tokens");
+  // a thread takes at least one element and one head
+  TORCH_CHECK((double)a.tokens * (a.Hq + a.Hk) * (double)D < 256. * kMaxInt, who, ": too many tokens");
   check_launch(launch_rotary(a, type, V, interleaved, current_stream()), who);
   return {yq, yk};
 }
