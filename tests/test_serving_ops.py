@@ -492,8 +492,9 @@ def attend64(q, cache, mask, scale):
         # of a score in 32 bits: D products and sums, the scales, the shift; of its exponential a few more
         error = torch.where(seen, x.abs() @ torch.nan_to_num(k, 0, 0, 0).abs().transpose(-1, -2) * abs(scale), 0.0)
         ds = (D + 8) * step32 * 2 * (error.amax(-1, keepdim=True) if end else 0.0) + 16 * step32
-        # each probability is rounded to the type once, the result once; sums of `end` terms are in 32 bits
-        tol[b] = (step * (1 + 2**-6) + 2 * ds + 2 * (end + 64) * step32) * size + step * 1.01 * torch.nan_to_num(o, 0, 0, 0).abs()
+        # each probability is given as two operands, the second of which is rounded (half a step of half a step), the
+        # result is rounded once; sums of `end` terms are in 32 bits
+        tol[b] = (step**2 * (1 + 2**-6) + 2 * ds + 2 * (end + 64) * step32) * size + step * 1.01 * torch.nan_to_num(o, 0, 0, 0).abs()
         # an exponential below 2^-126 of the largest, which is 1, may be lost in 32 bits: at most that times its value
         tol[b] += (end * 2.0**-126 * v0.abs().amax() if end else 0.0) * (total > 0)
         if q.dtype == FP16:  # probabilities below its normal range: half of its least step, relative to the largest scale
@@ -1087,3 +1088,21 @@ def test_cache_attention_odd_tokens_reach_those_that_see_them(quant, T):
         cache.lengths.fill_(slot)
         cache.append(k[:, :, 2:3], v[:, :, 2:3])
         cache.lengths.fill_(600)
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 9])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_cache_attention_infinite_values_among_the_standing(T, dtype):
+    """Far from the new tokens, where no mask is: an infinity stays one, two of unlike signs and NaN are NaN."""
+    cache = filled_cache(2, 1, 1200, 64, [1100, 300], T, dtype, None, "cuda")
+    cache.v[:, :, 40, 1] = math.inf
+    cache.v[:, :, 50, 2] = -math.inf
+    cache.v[:, :, 60, 3] = math.nan
+    cache.v[:, :, 70, 4] = math.inf
+    cache.v[:, :, 200, 4] = -math.inf
+    q = randn(2, 4, T, 64, seed=78, dtype=dtype, device="cuda")
+    out = cache_attention(q, cache)
+    check_attention(out, q, cache, None)
+    assert (out[..., 1] == math.inf).all() and (out[..., 2] == -math.inf).all()
+    assert torch.isnan(out[..., 3:5]).all() and torch.isfinite(out[..., 5:]).all() and torch.isfinite(out[..., 0]).all()
