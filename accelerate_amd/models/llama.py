@@ -445,7 +445,7 @@ class LlamaForCausalLM(nn.Module):
         table = self.rope_cos.shape[0]
         if temperature < 0:
             raise ValueError(f"temperature must not be negative, got {temperature}")
-        if max_new_tokens < 1 or S < 1:
+        if max_new_tokens < 1 or S < 1 or B < 1:
             raise ValueError("generation needs a prompt and at least one new token")
         if S + max_new_tokens > table:
             raise ValueError(f"{S} + {max_new_tokens} tokens, the model has {table} positions")

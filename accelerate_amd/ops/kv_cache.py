@@ -44,7 +44,8 @@ class KVCache:
 
     ``quant`` is None (held in ``dtype``), "int8" or "fp8". ``lengths`` is an int32 tensor [B] that the layers of a
     model share; by default the cache makes its own, of zeros. ``k`` and ``v`` are views of what is held
-    ([B, H, max_len, D]), ``k_scale`` and ``v_scale`` ([B, H, max_len]) of the scales of an 8-bit cache.
+    ([B, H, max_len, D]), ``k_scale`` and ``v_scale`` ([B, H, max_len]) of the scales of an 8-bit cache (of "fp8" powers
+    of two: attention goes by their exponents).
     """
 
     def __init__(
@@ -81,8 +82,13 @@ class KVCache:
             self._v_scale = torch.zeros_like(self._k_scale)
         if lengths is None:
             lengths = torch.zeros(batch_size, dtype=torch.int32, device=self.device)
-        elif lengths.dtype != torch.int32 or lengths.shape != (batch_size,) or lengths.device != self.device:
-            raise ValueError(f"lengths must be an int32 tensor [{batch_size}] on {self.device}")
+        elif (
+            lengths.dtype != torch.int32
+            or lengths.shape != (batch_size,)
+            or lengths.device != self.device
+            or not lengths.is_contiguous()
+        ):
+            raise ValueError(f"lengths must be a contiguous int32 tensor [{batch_size}] on {self.device}")
         self.lengths = lengths
 
     @property
@@ -239,7 +245,8 @@ def cache_attention(
     ``mask[..., i, j]`` is true: a bool mask [T, W] or [B, T, W] over the W first new slots (a tree of drafted tokens:
     ``draft_tree_mask``). Without a mask query i sees the new slots 0..i. A query that sees nothing gets zeros. The
     values of slots that a query does not see, NaN among them, do not reach it. ``scale`` defaults to 1 / sqrt(D).
-    There is no backward pass.
+    q is of the cache's type; an 8-bit cache takes bf16 and fp16. The result [B, Hq, T, D] is laid out [B, T, Hq, D] in
+    memory. There is no backward pass.
     """
     _no_grad("cache_attention", q)
     if scale is None:

@@ -110,7 +110,7 @@ def _rotary_reference(q, k, cos, sin, positions, interleaved):
         if not ok:
             raise RuntimeError(f"rotary_embedding: {message}")
 
-    need(q.dim() == 4, "q must be a [B, H, S, D] tensor")
+    need(q.dim() == 4 and q.is_floating_point(), "q must be a [B, H, S, D] tensor of floats")
     B, _, S, D = q.shape
     need(
         k is None or (k.dim() == 4 and k.dtype == q.dtype and (k.shape[0], *k.shape[2:]) == (B, S, D)),
@@ -135,7 +135,9 @@ def _rotary_reference(q, k, cos, sin, positions, interleaved):
         )
         at = positions.long().expand(B, S)
         known = ((at >= 0) & (at < cos.shape[0]))[:, None, :, None]
-        at = at.clamp(0, max(cos.shape[0] - 1, 0))
+        if cos.shape[0] == 0:  # no position is known
+            cos = sin = cos.new_zeros(1, half)
+        at = at.clamp(0, cos.shape[0] - 1)
         c = torch.where(known, cos[at][:, None], float("nan"))
         s = torch.where(known, sin[at][:, None], float("nan"))
 

@@ -1106,3 +1106,20 @@ def test_cache_attention_infinite_values_among_the_standing(T, dtype):
     check_attention(out, q, cache, None)
     assert (out[..., 1] == math.inf).all() and (out[..., 2] == -math.inf).all()
     assert torch.isnan(out[..., 3:5]).all() and torch.isfinite(out[..., 5:]).all() and torch.isfinite(out[..., 0]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rotary_without_positions_in_the_tables(device):
+    empty = torch.empty(0, 4, device=device)
+    y = rotary_embedding(randn(1, 1, 2, 12, device=device), None, empty, empty, positions=torch.zeros(2, dtype=torch.long, device=device))
+    assert torch.isnan(y[..., :8]).all() and torch.isfinite(y[..., 8:]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_cache_refuses_odd_lengths(device):
+    with pytest.raises(ValueError):
+        KVCache(2, 1, 8, 32, device=device, lengths=torch.zeros(4, dtype=torch.int32, device=device)[::2])
+    cache = KVCache(2, 1, 8, 32, dtype=BF16, device=device)
+    cache.lengths.copy_(torch.tensor([-5, 1000]))  # behind the ends: as the nearest length
+    q = torch.ones(2, 1, 2, 32, dtype=BF16, device=device)
+    check_attention(cache_attention(q, cache), q, cache, None)
