@@ -258,14 +258,16 @@ class LlamaForCausalLM(nn.Module):
         elif isinstance(module, nn.Embedding):
             module.weight.data.normal_(mean=0.0, std=0.02)
 
-    def forward(self, input_ids, labels=None, kv_caches=None, positions=None, mask=None, offset=0, prefill=False):
+    def forward(
+        self, input_ids, labels=None, kv_caches=None, positions=None, mask=None, offset=0, prefill=False, rope=None
+    ):
         """``kv_caches`` are the dicts of ``make_kv_caches`` or the KVCaches of ``make_serving_caches``. The latter take
         the tokens behind those that stand (from ``offset`` on, at ``positions`` [B, T], each seeing what ``mask`` says:
-        see ``cache_attention``) and are not advanced; ``prefill`` says that nothing stands yet."""
+        see ``cache_attention``) and are not advanced; ``prefill`` says that nothing stands yet, ``rope`` are the
+        tables of ``serving_rope``, for callers of many steps."""
         x = self.embed_tokens(input_ids)
         if kv_caches is not None and isinstance(kv_caches[0], KVCache):
-            # a model cast to bf16 has cast its tables too; the kernel reads fp32
-            cos, sin = self.rope_cos.to(x.device).float(), self.rope_sin.to(x.device).float()
+            cos, sin = rope if rope is not None else self.serving_rope(x.device)
             if positions is None:
                 after = torch.arange(offset, offset + input_ids.shape[1], device=x.device)
                 positions = kv_caches[0].lengths.long()[:, None] + after
@@ -296,6 +298,10 @@ class LlamaForCausalLM(nn.Module):
             }
             for _ in range(c.num_hidden_layers)
         ]
+
+    def serving_rope(self, device):
+        """The rotary tables as the kernel reads them: on the device, and fp32 where the model was cast to bf16."""
+        return self.rope_cos.to(device).float(), self.rope_sin.to(device).float()
 
     def make_serving_caches(self, batch_size, max_len, device, dtype, quant=None, lengths=None):
         """A KVCache a layer (``quant`` None, "int8" or "fp8"); all share one tensor of lengths."""
@@ -479,6 +485,9 @@ class LlamaForCausalLM(nn.Module):
                 B, S + max_new_tokens + nodes, device, draft_model.lm_head.weight.dtype, cache_dtype, lengths
             )
 
+        rope = self.serving_rope(device)
+        draft_rope = draft_model.serving_rope(device) if draft_model is not None else None
+
         def numbers(n):
             if temperature == 0.0:
                 return torch.zeros(B, n, device=device)
@@ -489,17 +498,17 @@ class LlamaForCausalLM(nn.Module):
             return verify_draft(probs[:, None], root.new_zeros(B, 1), numbers(1)).tokens
 
         root = input_ids.new_zeros(B, 1)
-        logits = self(input_ids, kv_caches=caches, prefill=True)["logits"][:, -1]
+        logits = self(input_ids, kv_caches=caches, prefill=True, rope=rope)["logits"][:, -1]
         root = draw(self._target_probs(logits, temperature))
         if draft_model is not None:
-            draft_model(input_ids, kv_caches=draft_caches, prefill=True)
+            draft_model(input_ids, kv_caches=draft_caches, prefill=True, rope=draft_rope)
         caches[0].advance(S)
         said = [[t] for t in root[:, 0].tolist()]
 
         if graph_decode and device.type == "cuda" and max_new_tokens > 1:
 
             def step():
-                best = self(root, kv_caches=caches)["logits"].argmax(-1)
+                best = self(root, kv_caches=caches, rope=rope)["logits"].argmax(-1)
                 root.copy_(best)
                 caches[0].advance(1)
 
@@ -527,7 +536,7 @@ class LlamaForCausalLM(nn.Module):
             if draft_model is not None:
                 for i, (first, last) in enumerate(levels):
                     logits = draft_model(
-                        tokens[-1], kv_caches=draft_caches, mask=mask[first:last, :last], offset=first,
+                        tokens[-1], kv_caches=draft_caches, mask=mask[first:last, :last], offset=first, rope=draft_rope,
                         positions=positions[:, first:last].clamp(max=draft_model.rope_cos.shape[0] - 1),
                     )["logits"]
                     if last == nodes:
@@ -539,7 +548,7 @@ class LlamaForCausalLM(nn.Module):
                         tokens.append(logits.topk(draft_widths[i], -1).indices.flatten(1))
             tokens = torch.cat(tokens, 1)
             logits = self(
-                tokens, kv_caches=caches, mask=None if chain else mask, positions=positions.clamp(max=table - 1)
+                tokens, kv_caches=caches, mask=None if chain else mask, positions=positions.clamp(max=table - 1), rope=rope
             )["logits"]
             verdict = verify_draft(
                 self._target_probs(logits, temperature), tokens, numbers(nodes),

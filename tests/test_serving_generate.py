@@ -159,3 +159,14 @@ def test_generate_refuses():
     ):
         with pytest.raises(ValueError):
             target.generate(ids, **{"max_new_tokens": 8, **kwargs})
+
+
+@gpu
+def test_graph_decode_with_tables_left_on_the_host():
+    """A model that was built on the GPU has its rotary tables on the host still."""
+    target, _ = models("cuda")
+    ids = prompt("cuda")
+    want = target.generate(ids, max_new_tokens=6, cache_dtype="int8")
+    target.rope_cos, target.rope_sin = target.rope_cos.cpu(), target.rope_sin.cpu()
+    for graph_decode in (False, True):
+        assert torch.equal(target.generate(ids, max_new_tokens=6, cache_dtype="int8", graph_decode=graph_decode), want)
