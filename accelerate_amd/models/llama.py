@@ -512,21 +512,22 @@ class LlamaForCausalLM(nn.Module):
                 root.copy_(best)
                 caches[0].advance(1)
 
-            first, start = root.clone(), lengths.clone()
-            side = torch.cuda.Stream()
-            side.wait_stream(torch.cuda.current_stream())
-            with torch.cuda.stream(side):
-                step()
-            torch.cuda.current_stream().wait_stream(side)
-            root.copy_(first)
-            lengths.copy_(start)
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                step()
-            out = [input_ids, first]
-            for _ in range(max_new_tokens - 1):
-                graph.replay()
-                out.append(root.clone())
+            with torch.cuda.device(device):
+                first, start = root.clone(), lengths.clone()
+                side = torch.cuda.Stream()
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    step()
+                torch.cuda.current_stream().wait_stream(side)
+                root.copy_(first)
+                lengths.copy_(start)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    step()
+                out = [input_ids, first]
+                for _ in range(max_new_tokens - 1):
+                    graph.replay()
+                    out.append(root.clone())
             return torch.cat(out, dim=1)
 
         while min(len(s) for s in said) < max_new_tokens:

@@ -30,9 +30,9 @@
 // Measured: 32 sequences of 8000 to 16000 int8 tokens, 64 query heads on 8:
 // 155 us, 5.3 TB/s; one of 130001 bf16 tokens: 97 us, 5.5 TB/s (a large copy:
 // 5.1). One of 300: 8 us, the latency of a launch and three readings in turn.
-// Of 108 rows (27 drafted tokens, 4 heads a group) over 8 x 4000 e4m3 tokens:
-// 37 us, where the bytes would take 11; decoding, exponentials and products
-// take turns there, with two waves a SIMD.
+// Of 108 rows (27 drafted tokens, 4 heads a group) over 8 sequences of 2000 to
+// 4000 e4m3 tokens: 37 us, where the bytes would take 11; decoding, exponentials
+// and products take turns there, with two waves a SIMD.
 
 #include "serving.h"
 

@@ -279,7 +279,9 @@ void kv_cache_append(at::Tensor cache_k, at::Tensor cache_v, OptTensor k_scale, 
   a.offset = offset;
   a.T = (int)k.size(2);
   if (c.B == 0 || c.H == 0 || a.T == 0) return;
-  const at::Tensor in[2] = {rows16(k), rows16(v)};
+  // the cache's own rows would be written while others of them are read
+  const auto own = [&](const at::Tensor& t) { return t.is_alias_of(cache_k) || t.is_alias_of(cache_v); };
+  const at::Tensor in[2] = {rows16(own(k) ? k.clone() : k), rows16(own(v) ? v.clone() : v)};
   for (int i = 0; i < 2; ++i) {
     a.x[i] = in[i].data_ptr();
     a.sb[i] = in[i].stride(0);

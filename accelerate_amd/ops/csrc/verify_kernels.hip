@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
   __shared__ double p_of[kMaxNodes], test_of[kMaxNodes];  // taken iff test (times what is left) < p
   __shared__ int token_of[kMaxNodes], parent_of[kMaxNodes], without[kMaxNodes];
   __shared__ int path[kMaxNodes];
+  __shared__ bool again[kMaxNodes];
   __shared__ int s_last, s_residual, s_without, s_count;
   __shared__ int votes[2][kThreads / 64];
   __shared__ double sums[kThreads / 64];
@@ -137,16 +138,24 @@ __global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
       if (s_without) without[0] = token_of[first];
     }
     for (int i = tid; i < first; i += kThreads) path[i] = i;
-  } else if (tid == 0) {
+  } else {
+    // A token that an earlier sibling has: refused there, it has nothing left.
+    for (int i = tid; i < a.T; i += kThreads) {
+      const int token = token_of[i], parent = parent_of[i];
+      bool is = false;
+#pragma unroll 8
+      for (int j = 1; j < i; ++j) is |= (token_of[j] == token) & (parent_of[j] == parent);
+      again[i] = is;
+    }
+    __syncthreads();
+  }
+  if (a.parents && tid == 0) {
     // children come after their parents, so one pass in order is the walk
     int cur = 0, n = 0, count = 0;
     double left = 1.;
     path[0] = 0;
     for (int i = 1; i < a.T; ++i) {
-      if (parent_of[i] != cur) continue;
-      bool again = false;  // a token refused before has nothing left
-      for (int j = 0; j < n; ++j) again |= without[j] == token_of[i];
-      if (again) continue;
+      if (parent_of[i] != cur || again[i]) continue;
       if (test_of[i] * left < p_of[i]) {
         cur = i;
         n = 0;

@@ -215,7 +215,7 @@ class KVCache:
 
 def _quantise(x, quant):
     if quant is None:
-        return x, None
+        return x.clone(), None  # the cache's own rows may overlap those that are written
     wide = x.float()
     amax = wide.abs().amax(-1) if x.shape[-1] else wide.new_zeros(wide.shape[:-1])
     bad = ~torch.isfinite(wide).all(-1)

@@ -43,6 +43,11 @@ def rope_is_fusable(x, cos) -> bool:
 # half or interleaved pairs, tables scaled for long contexts.
 # ---------------------------------------------------------------------------
 
+_SCALING_KEYS = {
+    "rope_type", "type", "factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor",
+    "beta_fast", "beta_slow", "attention_factor",
+}
+
 
 def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[dict] = None):
     """(angle per position of each pair [rotary_dim / 2], factor of cos and sin), in 64 bits.
@@ -57,6 +62,8 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[
     - ``{"rope_type": "yarn", "factor", "original_max_position_embeddings"}``, with ``beta_fast`` (32) and
       ``beta_slow`` (1) turns as the ends of a ramp over the pairs, and ``attention_factor``
       (0.1 ln(factor) + 1) on cos and sin.
+
+    Other keys are refused: they would change the tables.
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
@@ -71,6 +78,9 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[
         return freq, 1.0
     if kind not in ("linear", "llama3", "yarn"):
         raise ValueError(f"unknown rope_type {kind!r}: linear, llama3 or yarn")
+    unknown = set(scaling) - _SCALING_KEYS
+    if unknown:
+        raise ValueError(f"unknown keys of the rotary scaling: {sorted(unknown)}")
     factor = float(scaling["factor"])
     if factor < 1:
         raise ValueError(f"the scaling factor must be at least 1, got {factor}")

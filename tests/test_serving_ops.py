@@ -862,6 +862,26 @@ def test_verify_views_and_empty(device):
     assert out.tokens.shape == (0, T) and out.counts.shape == (0,)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T", [1024, 300])
+def test_verify_wide_trees(device, T):
+    """All nodes are children of the root, a token twice among them, all but the last refused."""
+    g = torch.Generator().manual_seed(T)
+    V = 2000
+    order = torch.randperm(V, generator=g)
+    tokens = order[torch.arange(T) % (T - 100)].repeat(2, 1)  # the last 100 for the second time
+    tokens[1, -1] = order[-1]
+    parents = torch.zeros(T, dtype=torch.int64)
+    parents[0] = -1
+    target = torch.softmax(torch.randn(2, T, V, generator=g), -1)
+    u = torch.full((2, T), 0.9)
+    u[1, -1] = 0.0
+    args = [target, tokens, u, None, parents]
+    out = verify_draft(*[a if a is None else a.to(device) for a in args])
+    assert out.counts.tolist() == [0, 1] and out.path[1, 1] == T - 1
+    check_verdict(out, verify64(*args))
+
+
 def test_verify_keeps_the_targets_distribution():
     """Over all drafts and numbers of a small vocabulary, the first token is distributed as the target's row."""
     g = torch.Generator().manual_seed(82)
@@ -1123,3 +1143,25 @@ def test_cache_refuses_odd_lengths(device):
     cache.lengths.copy_(torch.tensor([-5, 1000]))  # behind the ends: as the nearest length
     q = torch.ones(2, 1, 2, 32, dtype=BF16, device=device)
     check_attention(cache_attention(q, cache), q, cache, None)
+
+
+def test_rope_scaling_refuses_what_it_does_not_know():
+    yarn = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096}
+    for more in ({"mscale": 1.0}, {"truncate": False}, {"rope_theta": 1e6}):
+        with pytest.raises(ValueError, match=next(iter(more))):
+            rope_frequencies(64, 1e4, {**yarn, **more})
+    rope_frequencies(64, 1e4, {**yarn, "beta_fast": 16, "beta_slow": 2, "attention_factor": 1.0})
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("offset", [0, 3])
+def test_append_of_the_caches_own_rows(device, offset):
+    g = torch.Generator().manual_seed(5)
+    cache = KVCache(2, 2, 300, 64, dtype=BF16, device=device)
+    k, v = torch.randn(2, 2, 2, 300, 64, generator=g).to(BF16).to(device)
+    cache.append(k, v)
+    cache.append(cache.k[:, :, 1:280], cache.v[:, :, 1:280], offset=offset)
+    for held, was in ((cache.k, k), (cache.v, v)):
+        assert torch.equal(held[:, :, offset : offset + 279], was[:, :, 1:280])
+        assert torch.equal(held[:, :, offset + 279 :], was[:, :, offset + 279 :])
+        assert torch.equal(held[:, :, :offset], was[:, :, :offset])
