@@ -658,7 +658,8 @@ __global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(Attend
 }
 
 // The splits of a row, joined, where they are few: D / 4 lanes a row, each of
-// four dimensions.
+// four dimensions. (With a workgroup a row, below, calls of 2 to 8 splits take
+// 1 us more, 6 where the rows are many: 8 x 8 x 108 rows.)
 template <typename T, int kD>
 __global__ void __launch_bounds__(256) attend_join_few_kernel(AttendArgs a) {
   constexpr int kLanes = kD / 4;

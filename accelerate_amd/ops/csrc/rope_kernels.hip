@@ -195,9 +195,11 @@ hipError_t launch_rotary(RotaryArgs a, ServingType type, int V, bool interleaved
   a.rotary_chunks = a.R / (2 * V);
   a.chunks = a.rotary_chunks + (a.D - a.R + 2 * V - 1) / (2 * V);
   const int heads = a.Hq + a.Hk;
-  // Few tokens: a thread for each head, the chip is not full anyway. Many: four
-  // heads a thread, with the table's values in its registers; 8192 tokens of
-  // 72 heads of 128 take 58 us, 65 with one head, 72 with nine.
+  // Few tokens: a thread for each head, the chip is not full anyway (400 tokens
+  // of 40 heads of 128 take 4.0 us, 5.6 with four heads; 819: 5.2 and 6.4; 1600:
+  // 8.7 and 8.7). Many: four heads a thread, with the table's values in its
+  // registers (3200: 13.0 us, 13.8 with one; 8192 of 72 heads 58 us, 65 with
+  // one, 72 with nine).
   const bool few = a.tokens * heads * a.chunks <= 256 * 1024;
   a.head_step = few ? heads : (heads + 3) / 4;
   switch (type) {
