@@ -4,6 +4,8 @@
 
 #include <torch/extension.h>
 #include <ATen/DeviceGuard.h>
+#include <ATen/ExpandUtils.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/hip/HIPStream.h>
 
@@ -42,6 +44,20 @@ hipStream_t current_stream() { return at::hip::getCurrentHIPStream().stream(); }
 
 void check_launch(hipError_t e, const char* who) {
   TORCH_CHECK(e == hipSuccess, who, " launch failed: ", hipGetErrorString(e));
+}
+
+// Memory on the device of a tensor, past the dispatcher: small calls are bound
+// by what the host does for them.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& as) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, as.device(), c10::nullopt));
+}
+
+// One like t, its last dimension contiguous where t's is.
+at::Tensor fresh_like(const at::Tensor& t) {
+  if (t.is_non_overlapping_and_dense())
+    return at::Tensor(at::detail::empty_strided_cuda(t.sizes(), t.strides(), t.scalar_type(), t.device()));
+  const auto strides = at::infer_dense_strides(t.sizes(), t.strides());
+  return at::Tensor(at::detail::empty_strided_cuda(t.sizes(), strides, t.scalar_type(), t.device()));
 }
 
 constexpr int64_t kMaxInt = std::numeric_limits<int>::max();
@@ -88,13 +104,13 @@ std::tuple<at::Tensor, OptTensor> rotate(at::Tensor q, OptTensor k, at::Tensor c
     a.pos_b = positions->dim() == 2 && positions->size(0) == B ? positions->stride(0) : 0;
   }
   if (q.stride(3) != 1) q = q.contiguous();
-  auto yq = at::empty_like(q);
-  if (yq.stride(3) != 1) yq = at::empty(q.sizes(), q.options());
+  auto yq = fresh_like(q);
+  if (yq.stride(3) != 1) yq = fresh(q.sizes(), q.scalar_type(), q);
   OptTensor yk;
   if (k.has_value()) {
     if (k->stride(3) != 1) k = k->contiguous();
-    yk = at::empty_like(*k);
-    if (yk->stride(3) != 1) yk = at::empty(k->sizes(), k->options());
+    yk = fresh_like(*k);
+    if (yk->stride(3) != 1) yk = fresh(k->sizes(), k->scalar_type(), q);
   }
   a.table_rows = cos_t.size(0);
   a.cos_t = cos_t.data_ptr<float>();
@@ -301,8 +317,8 @@ std::tuple<at::Tensor, at::Tensor> kv_cache_read(at::Tensor cache_k, at::Tensor 
                   length < kMaxInt / (2 * std::max<int64_t>(c.B, 1) * std::max<int64_t>(c.H, 1)),
               who, ": bad length ", length, " or offset ", offset);
   const c10::OptionalDeviceGuard guard(at::device_of(cache_k));
-  auto yk = at::empty({c.B, c.H, length, c.D}, cache_k.options().dtype(dtype));
-  auto yv = at::empty_like(yk);
+  auto yk = fresh({c.B, c.H, length, c.D}, dtype, cache_k);
+  auto yv = fresh({c.B, c.H, length, c.D}, dtype, cache_k);
   const ServingType out = type_of(yk, who, true);
   CacheArgs a{};
   fill_cache(a, c, cache_k, cache_v, k_scale, v_scale, max_len);
@@ -372,7 +388,8 @@ at::Tensor kv_cache_attend(at::Tensor q, at::Tensor cache_k, at::Tensor cache_v,
     a.mb = mask->dim() == 3 && mask->size(0) == c.B ? mask->stride(0) : 0;
   }
   // where the model reshapes [B, T, Hq * D] next, this is a view
-  auto out = at::empty({c.B, T, Hq, c.D}, q.options()).transpose(1, 2);
+  at::Tensor out(at::detail::empty_strided_cuda({c.B, Hq, T, c.D}, {T * Hq * c.D, c.D, Hq * c.D, 1}, q.scalar_type(),
+                                                q.device()));
   if (out.numel() == 0) return out;
   if (max_len == 0 && mask.has_value()) return out.zero_();  // nothing to see
   TORCH_CHECK(T <= max_len || mask.has_value(), who, ": ", T, " new tokens, the cache has ", max_len, " slots");
@@ -398,7 +415,7 @@ at::Tensor kv_cache_attend(at::Tensor q, at::Tensor cache_k, at::Tensor cache_v,
   at::Tensor part;
   if (a.splits > 1) {
     const int64_t parts = (int64_t)c.B * c.H * rows * a.splits;
-    part = at::empty({parts * (c.D + 2)}, q.options().dtype(at::kFloat));
+    part = fresh({parts * (c.D + 2)}, at::kFloat, q);
     a.part_o = part.data_ptr<float>();
     a.part_ml = a.part_o + parts * c.D;
   }
@@ -447,14 +464,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_draft(at::Tensor target, a
   if (target.stride(2) != 1) target = target.contiguous();
   tokens = tokens.contiguous();
   uniforms = uniforms.contiguous();
-  auto out_tokens = at::empty({B, T}, tokens.options());
-  auto counts = at::empty({B}, tokens.options());
-  auto path = at::empty({B, T}, tokens.options());
+  auto out_tokens = fresh({B, T}, at::kLong, tokens);
+  auto counts = fresh({B}, at::kLong, tokens);
+  auto path = fresh({B, T}, at::kLong, tokens);
   if (B == 0) return {out_tokens, counts, path};
   a.chunks = verify_chunks(V);
   const int64_t meta_ints = verify_meta_ints((int)T);
-  auto partial = at::empty({B, a.chunks}, target.options().dtype(at::kDouble));
-  auto meta = at::empty({B, meta_ints}, target.options().dtype(at::kInt));
+  const int64_t sums = B * a.chunks;
+  auto work = fresh({sums + (B * meta_ints + 1) / 2}, at::kDouble, target);  // the chunks' sums, then meta
   a.target = target.data_ptr();
   a.tb = target.stride(0);
   a.tt = target.stride(1);
@@ -466,8 +483,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_draft(at::Tensor target, a
   a.out_tokens = out_tokens.data_ptr<int64_t>();
   a.counts = counts.data_ptr<int64_t>();
   a.path = path.data_ptr<int64_t>();
-  a.partial = partial.data_ptr<double>();
-  a.meta = meta.data_ptr<int>();
+  a.partial = work.data_ptr<double>();
+  a.meta = reinterpret_cast<int*>(a.partial + sums);
   a.B = (int)B;
   a.T = (int)T;
   a.V = V;
