@@ -351,7 +351,6 @@ struct Rows : Shape<T, kKind, kD> {
     // The largest score is the largest product, so that only one a row has to
     // be scaled before the exponentials. A negative scale turns the queries.
     scale = fmaxf(fabsf(a.scale_log2), 0x1p-126f);  // not zero: times minus infinity that is NaN
-    const unsigned turn = !S::kScaled && a.scale_log2 < 0.f ? 0x80008000u : 0u;
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt) {
       const int row = min(row0 + mt * 16 + c, rows - 1);
@@ -360,12 +359,22 @@ struct Rows : Shape<T, kKind, kD> {
 #pragma unroll
       for (int ds = 0; ds < S::kQK; ++ds) {
         const int d = S::kPaired ? (ds / 2) * 64 + g * 16 + (ds & 1) * 8 : ds * 32 + g * 8;
-        q[mt][ds] = __builtin_bit_cast(OV, *reinterpret_cast<const uint4v*>(src + d) ^ turn);
+        q[mt][ds] = __builtin_bit_cast(OV, *reinterpret_cast<const uint4v*>(src + d));
       }
       m[mt] = kNothing;
       l[mt] = 0.f;
 #pragma unroll
       for (int j = 0; j < S::kND; ++j) o[mt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  __device__ __forceinline__ void turn(const AttendArgs& a) {
+    if constexpr (!S::kScaled) {
+      const unsigned sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+        for (int ds = 0; ds < S::kQK; ++ds) q[mt][ds] = __builtin_bit_cast(OV, __builtin_bit_cast(uint4v, q[mt][ds]) ^ sign);
     }
   }
 
@@ -569,13 +578,21 @@ __global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(Attend
   // conditional: a wave without keys, or without more, reads its last tile or
   // the sequence's first once more, from a cache. Registers that a branch may
   // leave unwritten were given away by the compiler while they were in use.
+  // The order of the first loads (queries, keys, values) is held fixed: the
+  // loop's waits are for the worst of its entries, and with the keys or the
+  // queries last each tile's values were waited for before its scores (32
+  // sequences of 8000 to 16000 int8 tokens: 154.9 us for 151.3).
   Tile<T, kKind, kD> tile;
   const int first = w.from + wave * kTile;
   const int safe = kOne ? min(first, a.slots - kTile) : first < w.stop ? first : 0;
-  tile.load_keys(keys, ks, safe, c, g);
-  tile.load_values(values, vs, safe, c, g);
   Rows<T, kKind, kD, kMT> rows;
   rows.start(a, w, row0, c, g);
+  __builtin_amdgcn_sched_barrier(0);
+  tile.load_keys(keys, ks, safe, c, g);
+  __builtin_amdgcn_sched_barrier(0);
+  tile.load_values(values, vs, safe, c, g);
+  __builtin_amdgcn_sched_barrier(0);
+  rows.turn(a);
   for (int key0 = first; key0 < w.stop; key0 += kStep) {
     const int next = key0 + kStep < w.stop ? key0 + kStep : key0;
     f32x4 s[kMT][2];
