@@ -147,16 +147,27 @@ __device__ __forceinline__ int clamped_length(const AttendArgs& a, int b) {
   return min(max(a.lengths[b], 0), a.max_len);
 }
 
-// how many splits of the grid have keys, and how many each has: the sequence's
-// own length is shared out in steps of a workgroup's keys, not the cache's
+// how many keys each split of the grid has: the sequence's own length is shared
+// out in steps of a workgroup's keys, not the cache's. Splits whose keys would
+// start behind all of them have none.
 struct Share {
-  int keys, active;
+  int steps, all;
+  __device__ __forceinline__ bool has(int split) const { return (int64_t)split * steps < all; }
 };
 
 __device__ __forceinline__ Share share_of(int end, const AttendArgs& a) {
   const int all = max(1, (end + kStep - 1) / kStep);
-  const int steps = (all + a.splits - 1) / a.splits;
-  return {steps * kStep, (all + steps - 1) / steps};
+  return {(int)a.by_splits.quotient(all + a.splits - 1), all};
+}
+
+// A row of a group: its token, and its head of all.
+struct RowOf {
+  int t, head;
+};
+
+__device__ __forceinline__ RowOf row_of(const AttendArgs& a, int h, int row) {
+  const int t = a.by_rep.quotient(row);
+  return {t, h * a.rep + row - t * a.rep};
 }
 
 // A row whose probabilities sum to zero saw nothing and is zero, or all that
@@ -186,13 +197,15 @@ __device__ __forceinline__ Work work_of(const AttendArgs& a) {
   w.rb = 0;
   if (a.row_blocks > 1) {
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
-    w.rb = at % a.row_blocks;
-    part = (at / a.row_blocks) * 8 + xcd;
+    const int of = a.by_row_blocks.quotient(at);
+    w.rb = at - of * a.row_blocks;
+    part = of * 8 + xcd;
   }
   w.any = part < parts;
-  w.split = part % splits;
-  w.bh = w.any ? part / splits : 0;
-  w.b = w.bh / a.Hkv;
+  const int bh = kOne ? part : a.by_splits.quotient(part);
+  w.split = part - bh * splits;
+  w.bh = w.any ? bh : 0;
+  w.b = a.by_heads.quotient(w.bh);
   w.h = w.bh - w.b * a.Hkv;
   w.n0 = clamped_length(a, w.b);
   w.end = (int)min((int64_t)w.n0 + a.W, (int64_t)a.max_len);
@@ -201,9 +214,10 @@ __device__ __forceinline__ Work work_of(const AttendArgs& a) {
     w.stop = w.end;
   } else {
     const Share share = share_of(w.end, a);
-    w.any = w.any && w.split < share.active;
-    w.from = w.split * share.keys;
-    w.stop = min(w.end, w.from + share.keys);
+    w.any = w.any && share.has(w.split);
+    const int64_t from = (int64_t)w.split * share.steps * kStep;
+    w.from = (int)from;
+    w.stop = (int)min((int64_t)w.end, from + share.steps * kStep);
   }
   return w;
 }
@@ -354,8 +368,8 @@ struct Rows : Shape<T, kKind, kD> {
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt) {
       const int row = min(row0 + mt * 16 + c, rows - 1);
-      const int t = row / a.rep, head = w.h * a.rep + row % a.rep;
-      const T* src = reinterpret_cast<const T*>(a.q) + w.b * a.qb + head * a.qh + t * a.qt;
+      const RowOf r = row_of(a, w.h, row);
+      const T* src = reinterpret_cast<const T*>(a.q) + w.b * a.qb + r.head * a.qh + r.t * a.qt;
 #pragma unroll
       for (int ds = 0; ds < S::kQK; ++ds) {
         const int d = S::kPaired ? (ds / 2) * 64 + g * 16 + (ds & 1) * 8 : ds * 32 + g * 8;
@@ -397,7 +411,7 @@ struct Rows : Shape<T, kKind, kD> {
       // condition was lost by the compiler.
 #pragma unroll
       for (int mt = 0; mt < kMT; ++mt) {
-        const int t_row = (row0 + mt * 16 + c) / a.rep;
+        const int t_row = a.by_rep.quotient(row0 + mt * 16 + c);
         // all of a lane's mask values are read at once, from inside the mask
         const bool chain = a.mask == nullptr;
         const uint8_t* bits = a.mask + w.b * a.mb + min(t_row, a.T - 1) * a.mt;
@@ -528,13 +542,13 @@ template <typename T, int N, bool kOne>
 __device__ __forceinline__ void write_row(const AttendArgs& a, const Work& w, int row, int d, const float* y, float top,
                                           float sum) {
   if (kOne || a.splits == 1) {
-    const int t = row / a.rep, head = w.h * a.rep + row % a.rep;
+    const RowOf r = row_of(a, w.h, row);
     const float inverse = 1.f / sum;
-    const float none = sum == 0.f ? empty_row(a, w.b, t, w.n0) : 0.f;
+    const float none = sum == 0.f ? empty_row(a, w.b, r.t, w.n0) : 0.f;
     struct alignas(N * 2 < 16 ? N * 2 : 16) { T v[N]; } out;
 #pragma unroll
     for (int j = 0; j < N; ++j) out.v[j] = (T)(sum == 0.f ? none : y[j] * inverse);
-    *reinterpret_cast<decltype(out)*>(reinterpret_cast<T*>(a.out) + w.b * a.ob + head * a.oh + t * a.ot + d) = out;
+    *reinterpret_cast<decltype(out)*>(reinterpret_cast<T*>(a.out) + w.b * a.ob + r.head * a.oh + r.t * a.ot + d) = out;
   } else {
     const int64_t at = ((int64_t)w.bh * a.T * a.rep + row) * a.splits + w.split;
     struct alignas(N * 4 < 16 ? N * 4 : 16) { float v[N]; } out;
@@ -557,9 +571,11 @@ __global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(Attend
   using S = Shape<T, kKind, kD>;
   using OV = typename Operand<T>::V;
   constexpr int kND = S::kND;
-  __shared__ float red[kWaves][4][kND][64];
+  constexpr int kV = kND < 4 ? kND : 4;
+  typedef float Some __attribute__((ext_vector_type(kV)));
+  __shared__ Some red[kWaves][kMT][4][kND / kV][64];
   __shared__ float red_m[kWaves][kMT][16], red_l[kWaves][kMT][16];
-  __shared__ int red_odd;
+  __shared__ int red_odd[kWaves];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -627,11 +643,11 @@ __global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(Attend
     tile.load_values(values, vs, next, c, g);
   }
 
-  // the four waves' parts of a row, joined
+  // The four waves' parts of a row, joined: wave i sums the elements r = i,
+  // neighbours of row c from (4 g + i) D / 16 on.
   rows.finish();
-  if (threadIdx.x == 0) red_odd = 0;
-  __syncthreads();
-  if (odd) red_odd = 1;
+  const bool wave_odd = __any(odd);
+  if (lane == 0) red_odd[wave] = wave_odd;
   if (g == 0) {
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt) {
@@ -639,36 +655,43 @@ __global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(Attend
       red_l[wave][mt][c] = rows.l[mt];
     }
   }
+#pragma unroll
+  for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < kND; j += kV) {
+        Some x;
+#pragma unroll
+        for (int i = 0; i < kV; ++i) x[i] = rows.o[mt][j + i][r];
+        red[wave][mt][r][j / kV][lane] = x;
+      }
   __syncthreads();
+  const bool any_odd = (red_odd[0] | red_odd[1] | red_odd[2] | red_odd[3]) != 0;
 #pragma unroll
   for (int mt = 0; mt < kMT; ++mt) {
     float top = kNothing, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) top = fmaxf(top, red_m[i][mt][c]);
+    float y[kND] = {};
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) sum += red_l[i][mt][c] * __builtin_amdgcn_exp2f(red_m[i][mt][c] - top);
-    const float mine = __builtin_amdgcn_exp2f(rows.m[mt] - top);
+    for (int i = 0; i < kWaves; ++i) {
+      const float weight = __builtin_amdgcn_exp2f(red_m[i][mt][c] - top);
+      sum += red_l[i][mt][c] * weight;
 #pragma unroll
-    for (int j = 0; j < kND; ++j)
+      for (int j = 0; j < kND; j += kV) {
+        const Some x = red[i][mt][wave][j / kV][lane];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) red[wave][r][j][lane] = rows.o[mt][j][r] * mine;
-    __syncthreads();
-    // wave i sums the elements r = i: neighbours of row c from (4 g + i) D / 16 on
-    const int row = row0 + mt * 16 + c;
-    float y[kND];
-#pragma unroll
-    for (int j = 0; j < kND; ++j) {
-      y[j] = 0.f;
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i) y[j] += red[i][wave][j][lane];
+        for (int e = 0; e < kV; ++e) y[j + e] += x[e] * weight;
+      }
     }
-    __syncthreads();
+    const int row = row0 + mt * 16 + c;
     if (row < a.T * a.rep) {
       const int d = (g * 4 + wave) * kND;
       bool nan = false;
 #pragma unroll
       for (int j = 0; j < kND; ++j) nan |= y[j] != y[j];
-      if (red_odd || (nan && sum == sum)) take_odd<T, kND>(a, w, row / a.rep, values, vs, d, y);
+      if (any_odd || (nan && sum == sum)) take_odd<T, kND>(a, w, a.by_rep.quotient(row), values, vs, d, y);
       write_row<T, kND, kOne>(a, w, row, d, y, top, sum);
     }
   }
@@ -684,18 +707,18 @@ __global__ void __launch_bounds__(256) attend_join_few_kernel(AttendArgs a) {
   const int lane = threadIdx.x % kLanes;
   const int64_t at_row = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   if (at_row >= (int64_t)a.B * a.Hkv * rows) return;
-  const int bh = (int)(at_row / rows), row = (int)(at_row - (int64_t)bh * rows);
-  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const int bh = a.by_rows.quotient((unsigned)at_row), row = (int)at_row - bh * rows;
+  const int b = a.by_heads.quotient(bh), h = bh - b * a.Hkv;
   const int n0 = clamped_length(a, b);
-  const int active = share_of((int)min((int64_t)n0 + a.W, (int64_t)a.max_len), a).active;
+  const Share share = share_of((int)min((int64_t)n0 + a.W, (int64_t)a.max_len), a);
   const float* ml = a.part_ml + at_row * a.splits * 2;
   const float* part = a.part_o + at_row * a.splits * kD + lane * 4;
   float m[kFewSplits], l[kFewSplits];
   f32x4 o[kFewSplits];
   float top = kNothing;
 #pragma unroll
-  for (int s = 0; s < kFewSplits; ++s) {  // splits behind the last repeat it, with no weight
-    const int at = min(s, active - 1);
+  for (int s = 0; s < kFewSplits; ++s) {  // in place of a split without keys the first, with no weight
+    const int at = s < a.splits && share.has(s) ? s : 0;
     m[s] = ml[at * 2];
     l[s] = ml[at * 2 + 1];
     o[s] = *reinterpret_cast<const f32x4*>(part + at * kD);
@@ -706,17 +729,17 @@ __global__ void __launch_bounds__(256) attend_join_few_kernel(AttendArgs a) {
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
     const float weight = __builtin_amdgcn_exp2f(m[s] - top);
-    const bool is = s < active;
+    const bool is = s < a.splits && share.has(s);
     sum += is ? l[s] * weight : 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] += is ? o[s][i] * weight : 0.f;
   }
-  const int t = row / a.rep, head = h * a.rep + row % a.rep;
-  const float none = sum == 0.f ? empty_row(a, b, t, n0) : 0.f, inverse = 1.f / sum;
+  const RowOf r = row_of(a, h, row);
+  const float none = sum == 0.f ? empty_row(a, b, r.t, n0) : 0.f, inverse = 1.f / sum;
   struct alignas(8) { T v[4]; } out;
 #pragma unroll
   for (int i = 0; i < 4; ++i) out.v[i] = (T)(sum == 0.f ? none : y[i] * inverse);
-  *reinterpret_cast<decltype(out)*>(reinterpret_cast<T*>(a.out) + b * a.ob + head * a.oh + t * a.ot + lane * 4) = out;
+  *reinterpret_cast<decltype(out)*>(reinterpret_cast<T*>(a.out) + b * a.ob + r.head * a.oh + r.t * a.ot + lane * 4) = out;
 }
 
 // Where they are many: a workgroup a row. Its threads take four
@@ -728,10 +751,10 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   __shared__ f32x4 red[kGroups][kLanes];
   __shared__ float weight[kMaxSplits], red_m[4], red_l[4];
   const int rows = a.T * a.rep, tid = threadIdx.x;
-  const int bh = blockIdx.x / rows, row = blockIdx.x - bh * rows;
-  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const int bh = a.by_rows.quotient(blockIdx.x), row = blockIdx.x - bh * rows;
+  const int b = a.by_heads.quotient(bh), h = bh - b * a.Hkv;
   const int n0 = clamped_length(a, b);
-  const int active = share_of((int)min((int64_t)n0 + a.W, (int64_t)a.max_len), a).active;
+  const Share share = share_of((int)min((int64_t)n0 + a.W, (int64_t)a.max_len), a);
   const int64_t at = (int64_t)blockIdx.x * a.splits;
 
   float m[kMaxSplits / 256], l[kMaxSplits / 256], top = kNothing;
@@ -740,7 +763,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
     const int s = tid + i * 256;
     m[i] = kNothing;
     l[i] = 0.f;
-    if (s < active) {
+    if (s < a.splits && share.has(s)) {
       m[i] = a.part_ml[(at + s) * 2];
       l[i] = a.part_ml[(at + s) * 2 + 1];
     }
@@ -768,16 +791,16 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   const float* part = a.part_o + at * kD + lane * 4;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = group; s < active; s += kGroups) y += *reinterpret_cast<const f32x4*>(part + (int64_t)s * kD) * weight[s];
+  for (int s = group; s < a.splits && share.has(s); s += kGroups) y += *reinterpret_cast<const f32x4*>(part + (int64_t)s * kD) * weight[s];
   red[group][lane] = y;
   __syncthreads();
   if (tid >= kD) return;
   float out = 0.f;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) out += red[i][tid / 4][tid % 4];
-  const int t = row / a.rep, head = h * a.rep + row % a.rep;
-  out = sum == 0.f ? empty_row(a, b, t, n0) : out / sum;
-  reinterpret_cast<T*>(a.out)[b * a.ob + head * a.oh + t * a.ot + tid] = (T)out;
+  const RowOf r = row_of(a, h, row);
+  out = sum == 0.f ? empty_row(a, b, r.t, n0) : out / sum;
+  reinterpret_cast<T*>(a.out)[b * a.ob + r.head * a.oh + r.t * a.ot + tid] = (T)out;
 }
 
 template <typename T, CacheKind kKind, int kD, bool kOne>
@@ -841,11 +864,17 @@ void plan_attend(AttendArgs& a) {
   const int rows = a.T * a.rep, per = rows <= 16 ? 16 : 32;
   a.row_blocks = (rows + per - 1) / per;
   a.splits = 1;
-  if (a.max_len <= kShort) return;
-  const int64_t groups = (int64_t)a.B * a.Hkv * a.row_blocks;
-  int64_t splits = (256 + groups - 1) / groups;
-  if (a.max_len / splits >= 2048) splits = (512 + groups - 1) / groups;
-  a.splits = (int)std::min<int64_t>(splits, (a.max_len + kStep - 1) / kStep);
+  if (a.max_len > kShort) {
+    const int64_t groups = (int64_t)a.B * a.Hkv * a.row_blocks;
+    int64_t splits = (256 + groups - 1) / groups;
+    if (a.max_len / splits >= 2048) splits = (512 + groups - 1) / groups;
+    a.splits = (int)std::min<int64_t>(splits, (a.max_len + kStep - 1) / kStep);
+  }
+  a.by_splits = Divisor(a.splits);
+  a.by_row_blocks = Divisor(a.row_blocks);
+  a.by_rep = Divisor(a.rep);
+  a.by_heads = Divisor(a.Hkv);
+  a.by_rows = Divisor(rows);
 }
 
 hipError_t launch_attend(const AttendArgs& a, ServingType type, CacheKind kind, hipStream_t stream) {

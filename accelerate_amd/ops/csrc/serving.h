@@ -47,6 +47,20 @@ struct CacheArgs {
   int heads_first;         // rows in the order of their heads, then tokens
 };
 
+// Division of numbers below 2^31 by one that the host knows: with l the bits of
+// d - 1, the quotient is (n + n m / 2^32) / 2^l, m = 2^32 (2^l - d) / d + 1.
+struct Divisor {
+  unsigned multiplier = 1, shift = 0;
+  Divisor() = default;
+  explicit Divisor(unsigned d) {
+    while ((1ull << shift) < d) ++shift;
+    multiplier = (unsigned)((((1ull << shift) - d) << 32) / d + 1);
+  }
+  __host__ __device__ unsigned quotient(unsigned n) const {
+    return (n + (unsigned)(((uint64_t)n * multiplier) >> 32)) >> shift;
+  }
+};
+
 struct AttendArgs {
   const void *q, *k, *v;
   const float *k_scale, *v_scale;
@@ -56,7 +70,8 @@ struct AttendArgs {
   float *part_o, *part_ml;     // [B * Hkv, rows, splits, D] and [.., 2]
   int64_t qb, qh, qt, ob, oh, ot, mb, mt;
   int B, Hkv, rep, T, W, D, slots, max_len;
-  int splits, row_blocks;      // set by plan_attend
+  int splits, row_blocks;      // set by plan_attend, as are
+  Divisor by_splits, by_row_blocks, by_rep, by_heads, by_rows;
   float scale_log2;            // the softmax scale times log2(e)
 };
 
