@@ -28,11 +28,12 @@
 // and sequences to fill the chip; a second kernel joins the parts.
 //
 // Measured: 32 sequences of 8000 to 16000 int8 tokens, 64 query heads on 8:
-// 155 us, 5.3 TB/s; one of 130001 bf16 tokens: 97 us, 5.5 TB/s (a large copy:
-// 5.1). One of 300: 8 us, the latency of a launch and three readings in turn.
+// 151 us, 5.4 TB/s; one of 130001 bf16 tokens: 93 us, 5.7 TB/s (a large copy:
+// 5.1). One of 300: 7.7 us, the latency of a launch and three readings in turn.
 // Of 108 rows (27 drafted tokens, 4 heads a group) over 8 sequences of 2000 to
-// 4000 e4m3 tokens: 37 us, where the bytes would take 11; decoding, exponentials
-// and products take turns there, with two waves a SIMD.
+// 4000 e4m3 tokens: 36 us, where the bytes would take 11: two waves a SIMD take
+// about 1600 cycles a tile (1130 of vector and 770 of matrix instructions, which
+// overlap in part), and the start, the end and the join 12 us.
 
 #include "serving.h"
 
@@ -564,8 +565,9 @@ __device__ __forceinline__ void write_row(const AttendArgs& a, const Work& w, in
 
 // The four waves of a workgroup take tiles of keys in turn, all for the same
 // 16 kMT rows, and join in the end. Where a short cache's keys are all one
-// workgroup's (kOne) the first tiles are loaded before the length is known: 300
-// keys take 8.1 us for 8.5. (Eight waves take 9.1.)
+// workgroup's (kOne) the first tiles are loaded before the length is known, which
+// took 0.4 us off 300 keys. (Eight waves there: 300 keys of 8 heads 7.9 us for
+// 7.7, 510 10.2 for 9.0, of 64 sequences 26.5 for 23.3.)
 template <typename T, CacheKind kKind, int kD, int kMT, bool kOne>
 __global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(AttendArgs a) {
   using S = Shape<T, kKind, kD>;
@@ -852,14 +854,16 @@ hipError_t attend_by_kind(const AttendArgs& a, CacheKind kind, hipStream_t strea
 // Splits of the keys: the host does not know the lengths, so the cache's size
 // stands for them; a shorter sequence is shared out over the same number, as
 // far as its steps go.
-//  * Up to 4 steps there is one, and no second launch (300 keys: 6.7 to 8.2 us
-//    with one, 7.5 to 8.1 with three; the host issues one in 7 us, two in 10).
-//  * Else one workgroup a CU: 16000 keys of 8 heads take 17.5 (bf16) and 13.0
-//    us (int8) with 32 splits, 19.4 and 14.4 with 64.
-//  * Two, where the parts stay long: then the second hides what the first
-//    waits for, and sequences of unlike length even out (130000 int8 keys of 8
-//    heads: 54.6 us with 32, 47.5 with 64; 32 sequences of up to 16000: 199 and
-//    156 us with one and two).
+//  * Up to 4 steps there is one, and no second launch (300 keys of 8 heads: 7.7
+//    us bf16 and 6.0 e4m3 with one, 7.9 and 7.3 with three; 500: 9.0 and 6.9, 8.0
+//    and 7.2 with four; a second launch takes the host 3 us more).
+//  * Else one workgroup a CU: 16000 keys of 8 heads take 17.3 (bf16) and 11.8
+//    us (int8) with 32 splits, 19.1 and 14.1 with 64; 130000 95.0 and 46.8, 96.4
+//    and 48.3.
+//  * Two for several sequences whose parts stay long: those of unlike length
+//    even out (32 of 8000 to 16000 int8 keys: 160.8 us with one, 150.3 with two;
+//    16 of 15000 to 30000, 2 heads of 64: 31.7 and 27.5. Equal lengths take up to
+//    5 % longer: 32 of 16000 174 and 182).
 void plan_attend(AttendArgs& a) {
   const int rows = a.T * a.rep, per = rows <= 16 ? 16 : 32;
   a.row_blocks = (rows + per - 1) / per;
@@ -867,7 +871,7 @@ void plan_attend(AttendArgs& a) {
   if (a.max_len > kShort) {
     const int64_t groups = (int64_t)a.B * a.Hkv * a.row_blocks;
     int64_t splits = (256 + groups - 1) / groups;
-    if (a.max_len / splits >= 2048) splits = (512 + groups - 1) / groups;
+    if (a.B > 1 && a.max_len / splits >= 2048) splits = (512 + groups - 1) / groups;
     a.splits = (int)std::min<int64_t>(splits, (a.max_len + kStep - 1) / kStep);
   }
   a.by_splits = Divisor(a.splits);
