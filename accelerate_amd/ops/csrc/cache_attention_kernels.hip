@@ -23,7 +23,8 @@
 //    j, j + D / 16, ...: the transposition of V is a choice of elements.
 //  * 8-bit codes are exact in bf16 and fp16, e4m3 codes times their scale (a
 //    power of two) in bf16. Other scales multiply, in 32 bits, the scores (the
-//    keys') and the probabilities (the values').
+//    keys') and the probabilities (the values'). Probabilities times scales
+//    need more than fp16's range, so those values are operands in bf16 then.
 // The cache's length is split over workgroups where there are too few heads
 // and sequences to fill the chip; a second kernel joins the parts.
 //
@@ -34,6 +35,8 @@
 // 4000 e4m3 tokens: 36 us, where the bytes would take 11: two waves a SIMD take
 // about 1600 cycles a tile (1130 of vector and 770 of matrix instructions, which
 // overlap in part), and the start, the end and the join 12 us.
+
+#include <type_traits>
 
 #include "serving.h"
 
@@ -230,6 +233,7 @@ struct Shape {
   // Other scales multiply scores and probabilities, in 32 bits.
   static constexpr bool kFolded = kKind == CacheKind::kFp8 && __is_same(T, __bf16);
   static constexpr bool kScaled = !kSame && !kFolded;
+  typedef std::conditional_t<kScaled, __bf16, T> VT;  // of the second product's operands
   static constexpr int kBytes = kSame ? 2 : 1;
   static constexpr int kRowBytes = kD * kBytes;
   static constexpr int kQK = kD / 32;  // products a tile of 16 keys
@@ -245,6 +249,8 @@ template <typename T, CacheKind kKind, int kD>
 struct Tile : Shape<T, kKind, kD> {
   using S = Shape<T, kKind, kD>;
   using OV = typename Operand<T>::V;
+  using VT = typename S::VT;
+  using VOV = typename Operand<VT>::V;
   static constexpr int kLoad = S::kSame || S::kPaired ? 16 : 8;
   static constexpr int kLoads = S::kPaired ? S::kQK / 2 : S::kQK;
   Raw<kLoad> k[2][kLoads];
@@ -287,13 +293,13 @@ struct Tile : Shape<T, kKind, kD> {
   }
 
   // Operands j and j + 1: the j-th and next values of the lane's eight keys.
-  __device__ __forceinline__ void value2(int j, OV& x, OV& y) const {
+  __device__ __forceinline__ void value2(int j, VOV& x, VOV& y) const {
     uint4v lo, hi;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       if constexpr (S::kScaled) {
-        lo[e / 2] = decode_bytes<T, kKind>(v[e].w[j / 4], v[e + 1].w[j / 4], j & 3);
-        hi[e / 2] = decode_bytes<T, kKind>(v[e].w[j / 4], v[e + 1].w[j / 4], (j & 3) + 1);
+        lo[e / 2] = decode_bytes<VT, kKind>(v[e].w[j / 4], v[e + 1].w[j / 4], j & 3);
+        hi[e / 2] = decode_bytes<VT, kKind>(v[e].w[j / 4], v[e + 1].w[j / 4], (j & 3) + 1);
       } else {
         unsigned a, b;
         if constexpr (S::kSame) {
@@ -310,8 +316,8 @@ struct Tile : Shape<T, kKind, kD> {
         hi[e / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
       }
     }
-    x = __builtin_bit_cast(OV, lo);
-    y = __builtin_bit_cast(OV, hi);
+    x = __builtin_bit_cast(VOV, lo);
+    y = __builtin_bit_cast(VOV, hi);
   }
 
   // A probability of zero does not hide an infinite or NaN value. In a tile
@@ -350,19 +356,20 @@ template <typename T, CacheKind kKind, int kD, int kMT>
 struct Rows : Shape<T, kKind, kD> {
   using S = Shape<T, kKind, kD>;
   using OV = typename Operand<T>::V;
-  // 8-bit values times probabilities would be lost below fp16's range
-  static constexpr bool kUnits = S::kScaled && __is_same(T, _Float16);
+  using VT = typename S::VT;
+  using VOV = typename Operand<VT>::V;
+  // Probabilities of at most 1 use fp16's range from below alone: they are
+  // operands in units of 2^-15, and what is lost then is below 2^-40.
+  static constexpr float kLift = __is_same(VT, _Float16) ? 0x1p15f : 1.f;
   OV q[kMT][S::kQK];
   f32x4 o[kMT][S::kND];
   float m[kMT], l[kMT];
   float scale;  // of the scores where the keys' are none, not negative
-  int unit;     // o is held in units of 2^unit (kUnits)
 
   __device__ __forceinline__ void start(const AttendArgs& a, const Work& w, int row0, int c, int g) {
     // Rows behind the last repeat it; no row reaches another's result, and
     // they are not written.
     const int rows = a.T * a.rep;
-    unit = -126;
     // The largest score is the largest product, so that only one a row has to
     // be scaled before the exponentials. A negative scale turns the queries.
     scale = fmaxf(fabsf(a.scale_log2), 0x1p-126f);  // not zero: times minus infinity that is NaN
@@ -397,7 +404,7 @@ struct Rows : Shape<T, kKind, kD> {
   // follow the maximum.
   __device__ __forceinline__ void soften(const AttendArgs& a, const Work& w, const f32x4 (&s)[kMT][2],
                                          const f32x4* kscale, const f32x4* vscale, int key0, int row0, int c, int g,
-                                         OV (&pv)[kMT][2]) {
+                                         VOV (&pv)[kMT][2]) {
     const bool masked = key0 + kTile > w.n0;  // the tile has slots that some rows do not see
     bool grew = false;
     float p[kMT][8], keep[kMT];
@@ -450,22 +457,6 @@ struct Rows : Shape<T, kKind, kD> {
       l[mt] = l[mt] * keep[mt] + sum;
     }
 
-    float unit_scale = 1.f;
-    if constexpr (kUnits) {
-      // Probabilities are held relative to the power of two of the largest
-      // scale so far, which is the same for all rows.
-      float most = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, vscale[e >> 2][e & 3]);
-      most = max_over_groups(most);
-      const int wanted = min(max(unit, (int)(__float_as_uint(most) >> 23) - 126), 120);
-      const float less = __builtin_ldexpf(1.f, max(unit - wanted, -126));
-      grew |= wanted > unit;
-#pragma unroll
-      for (int mt = 0; mt < kMT; ++mt) keep[mt] *= less;
-      unit = wanted;
-      unit_scale = __builtin_ldexpf(1.f, -unit);
-    }
     if (__any(grew)) {
 #pragma unroll
       for (int mt = 0; mt < kMT; ++mt)
@@ -477,7 +468,8 @@ struct Rows : Shape<T, kKind, kD> {
     // that left out. One alone adds half a step of the type a key to the
     // result's own (an error of 0.0023 of random bf16 values, 0.0017 with two).
     // The second product costs nothing where the reading of the keys bounds,
-    // and 3 to 6 % at 108 rows.
+    // and 3 to 6 % at 108 rows. Two of bf16 hold 16 bits of a probability, two
+    // of fp16 22, where the result has 8 or 11.
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt) {
       uint4v x, rest;
@@ -485,15 +477,18 @@ struct Rows : Shape<T, kKind, kD> {
       for (int e = 0; e < 8; e += 2) {
         float p0 = p[mt][e], p1 = p[mt][e + 1];
         if constexpr (S::kScaled) {
-          p0 *= vscale[e >> 2][e & 3] * unit_scale;
-          p1 *= vscale[e >> 2][(e & 3) + 1] * unit_scale;
+          p0 *= vscale[e >> 2][e & 3];
+          p1 *= vscale[e >> 2][(e & 3) + 1];
+        } else if constexpr (kLift != 1.f) {
+          p0 *= kLift;
+          p1 *= kLift;
         }
-        x[e / 2] = pack2<T>(p0, p1);
-        const f32x2 is = unpack2<T>(x[e / 2]);
-        rest[e / 2] = pack2<T>(p0 - is[0], p1 - is[1]);
+        x[e / 2] = pack2<VT>(p0, p1);
+        const f32x2 is = unpack2<VT>(x[e / 2]);
+        rest[e / 2] = pack2<VT>(p0 - is[0], p1 - is[1]);
       }
-      pv[mt][0] = __builtin_bit_cast(OV, x);
-      pv[mt][1] = __builtin_bit_cast(OV, rest);
+      pv[mt][0] = __builtin_bit_cast(VOV, x);
+      pv[mt][1] = __builtin_bit_cast(VOV, rest);
     }
   }
 
@@ -502,10 +497,9 @@ struct Rows : Shape<T, kKind, kD> {
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt) {
       l[mt] = sum_over_groups(l[mt]);
-      if constexpr (kUnits) {
-        const float one = __builtin_ldexpf(1.f, unit);
+      if constexpr (kLift != 1.f) {
 #pragma unroll
-        for (int j = 0; j < S::kND; ++j) o[mt][j] *= one;
+        for (int j = 0; j < S::kND; ++j) o[mt][j] *= 1.f / kLift;
       }
     }
   }
@@ -572,6 +566,8 @@ template <typename T, CacheKind kKind, int kD, int kMT, bool kOne>
 __global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(AttendArgs a) {
   using S = Shape<T, kKind, kD>;
   using OV = typename Operand<T>::V;
+  using VT = typename S::VT;
+  using VOV = typename Operand<VT>::V;
   constexpr int kND = S::kND;
   constexpr int kV = kND < 4 ? kND : 4;
   typedef float Some __attribute__((ext_vector_type(kV)));
@@ -628,18 +624,18 @@ __global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(Attend
     const f32x4 kscale[2] = {tile.kscale[0], tile.kscale[1]};
     tile.load_keys(keys, ks, next, c, g);
     if (key0 + kTile > w.n0) odd |= tile.clear(key0, w.end, g);
-    OV pv[kMT][2];
+    VOV pv[kMT][2];
     rows.soften(a, w, s, kscale, tile.vscale, key0, row0, c, g, pv);
 #pragma unroll
     for (int j = 0; j < kND; j += 2) {
-      OV v0, v1;
+      VOV v0, v1;
       tile.value2(j, v0, v1);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt) {
-          rows.o[mt][j] = Operand<T>::mfma(v0, pv[mt][i], rows.o[mt][j]);
-          rows.o[mt][j + 1] = Operand<T>::mfma(v1, pv[mt][i], rows.o[mt][j + 1]);
+          rows.o[mt][j] = Operand<VT>::mfma(v0, pv[mt][i], rows.o[mt][j]);
+          rows.o[mt][j + 1] = Operand<VT>::mfma(v1, pv[mt][i], rows.o[mt][j + 1]);
         }
     }
     tile.load_values(values, vs, next, c, g);

@@ -1,0 +1,73 @@
+"""Serving operators where a value, a weight or a call is extreme: small weights, infinities, types, refusals."""
+
+import math
+
+import pytest
+import torch
+
+from accelerate_amd.ops import KVCache, cache_attention
+
+gpu = pytest.mark.gpu
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+# ---- attention: weights far below the largest -----------------------------------------------------------------------
+
+
+def sink_cache(B, H, n, D, quant, sink_value, gap, others):
+    """n tokens, one of which (the 7th) has a score higher by `gap` powers of two than the others', which are alike; its
+    value is `sink_value`, theirs are `others` [n, D]. Returns the cache, the last token not advanced over, and a query."""
+    cache = KVCache(B, H, n, D, dtype=FP16, quant=quant, device="cuda")
+    k, v = torch.zeros(1, 1, n, D, dtype=FP16), others.to(FP16).expand(1, 1, n, D).clone()
+    k[..., 7, 0], v[..., 7, :] = 8.0, sink_value
+    cache.append(k.expand(B, H, n, D).cuda(), v.expand(B, H, n, D).cuda())
+    cache.lengths.fill_(n - 1)
+    q = torch.zeros(B, H, 1, D, dtype=FP16)
+    q[..., 0] = gap * math.log(2)
+    return cache, q.cuda()
+
+
+def check_weighted(out, q, cache, scale):
+    """Against the definition in 64 bits, with what the cache holds."""
+    n = cache.max_len
+    k, v = (x[0, 0].double().cpu() for x in cache.read(dtype=FP32))
+    s = k @ q[0, 0, 0].double().cpu() * scale
+    p = torch.exp(s - s.max())
+    total = p.sum()
+    want, size = p @ v / total, p @ v.abs() / total
+    # A score has one product that is not zero: it and its scales are rounded four times, its difference to the largest
+    # once, its exponential to 2 steps (of 32 bits). A probability is held in 16 bits at least, and one below 2^-40 of
+    # the largest may be lost. Sums of n terms are in 32 bits.
+    score = 6 * half_step(FP32) * s.abs().max() + 4 * half_step(FP32)
+    tolerance = (2**-16 * 1.01 + 2 * score + 2 * (n + 64) * half_step(FP32)) * size
+    tolerance += n * 2.0**-40 * v.abs().max() / total
+    tolerance += half_step(FP16) * 1.01 * want.abs() + 2.0**-25  # the result's own rounding
+    got = out.double().cpu()
+    assert torch.equal(got, got[:1, :1].expand_as(got))
+    error = (got[0, 0, 0] - want).abs()
+    assert (error <= tolerance).all(), (error / tolerance).max()
+
+
+@gpu
+@pytest.mark.parametrize("quant", [None, "int8", "fp8"])
+@pytest.mark.parametrize("gap", [20.0, 24.5, 26.0, 30.0])
+@pytest.mark.parametrize("B, n", [(1, 500), (1, 2000), (64, 1500)])
+def test_weights_far_below_the_largest_count_in_fp16(quant, gap, B, n):
+    """One token without a value takes nearly all the weight: the result is what the others' small weights sum to."""
+    g = torch.Generator().manual_seed(1)
+    cache, q = sink_cache(B, 4, n, 64, quant, 0.0, gap, (torch.rand(n, 64, generator=g) + 1) * 15000)
+    check_weighted(cache_attention(q, cache, scale=0.125), q, cache, 0.125)
+
+
+@gpu
+@pytest.mark.parametrize("quant", [None, "int8", "fp8"])
+@pytest.mark.parametrize("gap", [-12.0, -30.0])
+def test_a_large_value_of_low_weight_leaves_the_others_their_bits_in_fp16(quant, gap):
+    g = torch.Generator().manual_seed(2)
+    cache, q = sink_cache(1, 4, 300, 64, quant, 30000.0, gap, torch.randn(300, 64, generator=g) * 0.01)
+    check_weighted(cache_attention(q, cache, scale=0.125), q, cache, 0.125)
