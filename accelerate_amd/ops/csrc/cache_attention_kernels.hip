@@ -695,6 +695,10 @@ __global__ void __launch_bounds__(256, (kD == 256 ? 1 : 2)) attend_kernel(Attend
   }
 }
 
+// A split's part of a sum. One that is infinite or NaN is the sum's, however
+// little the split weighs: its weight may be zero in 32 bits.
+__device__ __forceinline__ float weighted(float x, float weight) { return __builtin_isfinite(x) ? x * weight : x; }
+
 // The splits of a row, joined, where they are few: D / 4 lanes a row, each of
 // four dimensions. (With a workgroup a row, below, calls of 2 to 8 splits take
 // 1 us more, 6 where the rows are many: 8 x 8 x 108 rows.)
@@ -730,7 +734,7 @@ __global__ void __launch_bounds__(256) attend_join_few_kernel(AttendArgs a) {
     const bool is = s < a.splits && share.has(s);
     sum += is ? l[s] * weight : 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] += is ? o[s][i] * weight : 0.f;
+    for (int i = 0; i < 4; ++i) y[i] += is ? weighted(o[s][i], weight) : 0.f;
   }
   const RowOf r = row_of(a, h, row);
   const float none = sum == 0.f ? empty_row(a, b, r.t, n0) : 0.f, inverse = 1.f / sum;
@@ -789,7 +793,11 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   const float* part = a.part_o + at * kD + lane * 4;
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = group; s < a.splits && share.has(s); s += kGroups) y += *reinterpret_cast<const f32x4*>(part + (int64_t)s * kD) * weight[s];
+  for (int s = group; s < a.splits && share.has(s); s += kGroups) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(part + (int64_t)s * kD);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] += weighted(x[i], weight[s]);
+  }
   red[group][lane] = y;
   __syncthreads();
   if (tid >= kD) return;

@@ -282,8 +282,8 @@ def cache_attention(
     p = torch.where(seen, p, 0.0)
     finite = torch.isfinite(v)
     out = p @ torch.where(finite, v, 0.0)
-    if not finite.all():  # of the slots that a query sees
-        odd = torch.where(finite, 0.0, v)[:, :, None] * p[..., None]
+    if not finite.all():  # of the slots that a query sees, however little they weigh
+        odd = torch.where(finite, 0.0, v)[:, :, None]
         out = out + torch.where(seen[..., None], odd, 0.0).sum(-2)
     return torch.where(seen.any(-1, keepdim=True), out, 0.0).to(q.dtype)
 

@@ -71,3 +71,26 @@ def test_a_large_value_of_low_weight_leaves_the_others_their_bits_in_fp16(quant,
     g = torch.Generator().manual_seed(2)
     cache, q = sink_cache(1, 4, 300, 64, quant, 30000.0, gap, torch.randn(300, 64, generator=g) * 0.01)
     check_weighted(cache_attention(q, cache, scale=0.125), q, cache, 0.125)
+
+
+# ---- attention: infinities ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("B, H, max_len", [(1, 1, 300), (1, 1, 4096), (16, 4, 1300)])  # one workgroup a head; many splits; few
+def test_an_infinite_value_of_no_weight_stays_infinite(device, B, H, max_len):
+    """A token far behind has a score 184 powers of two above the others': their weights are zero in 32 bits."""
+    n, D = max_len - 20, 64
+    cache = KVCache(B, H, max_len, D, dtype=BF16, device=device)
+    cache.v.fill_(1)
+    cache.k[:, :, n - 100, 0] = 64.0
+    cache.v[:, :, 3, 1], cache.v[:, :, 4, 2], cache.v[:, :, 5, 3] = math.inf, -math.inf, math.nan
+    cache.v[:, :, 6, 4], cache.v[:, :, 140, 4] = math.inf, -math.inf
+    cache.lengths.fill_(n - 1)
+    q = torch.zeros(B, 2 * H, 1, D, dtype=BF16, device=device)
+    q[:, ::2, :, 0] = 16.0  # every other head: 64 * 16 / 8 / ln 2
+    out = cache_attention(q, cache).float().cpu()
+    assert (out[..., 1] == math.inf).all() and (out[..., 2] == -math.inf).all() and torch.isnan(out[..., 3:5]).all()
+    # the others are means of ones: sums of n terms in 32 bits, and the result's own rounding
+    rest = out[..., [0, *range(5, D)]]
+    assert ((rest - 1).abs() <= half_step(BF16) + 2 * (n + 64) * half_step(FP32)).all()
