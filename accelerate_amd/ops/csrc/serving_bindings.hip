@@ -60,6 +60,11 @@ at::Tensor fresh_like(const at::Tensor& t) {
   return at::Tensor(at::detail::empty_strided_cuda(t.sizes(), strides, t.scalar_type(), t.device()));
 }
 
+// A forward-mode derivative of a tensor, which the kernels would drop.
+void check_not_dual(const at::Tensor& t, const char* who) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), who, " has no forward-mode derivative on the GPU");
+}
+
 constexpr int64_t kMaxInt = std::numeric_limits<int>::max();
 
 }  // namespace
@@ -71,6 +76,7 @@ std::tuple<at::Tensor, OptTensor> rotate(at::Tensor q, OptTensor k, at::Tensor c
   const char* who = "rotary_embedding";
   TORCH_CHECK(q.is_cuda() && q.dim() == 4, who, ": q must be a [B, H, S, D] tensor on the GPU");
   const ServingType type = type_of(q, who, true);
+  for (const at::Tensor* t : {&q, k.has_value() ? &*k : &q, &cos_t, &sin_t}) check_not_dual(*t, who);
   const int64_t B = q.size(0), S = q.size(2), D = q.size(3);
   if (k.has_value()) {
     check_device(*k, q, who, "k");

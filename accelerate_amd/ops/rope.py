@@ -175,7 +175,8 @@ def rotary_embedding(
     rotated, the rest is copied; pair i is the elements (i, i + R / 2), or (2 i, 2 i + 1) where ``interleaved``.
     ``positions`` is int64 or int32, [S] or [B, S]; None means 0..S-1. A token whose position the tables do not
     have gets NaN in its rotated elements. bf16, fp16 and fp32, any strides (transposed views are read in
-    place). The gradient of q and k is the rotation back; the tables have none.
+    place). The gradient of q and k is the rotation back; the tables have none. Forward-mode derivatives are refused
+    on the GPU.
     """
     if q.is_cuda:
         out = _load_extension(required=True).rotary(q, k, cos, sin, positions, interleaved)

@@ -4,8 +4,9 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from accelerate_amd.ops import KVCache, cache_attention
+from accelerate_amd.ops import KVCache, cache_attention, rope_tables, rotary_embedding
 
 gpu = pytest.mark.gpu
 DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
@@ -94,3 +95,31 @@ def test_an_infinite_value_of_no_weight_stays_infinite(device, B, H, max_len):
     # the others are means of ones: sums of n terms in 32 bits, and the result's own rounding
     rest = out[..., [0, *range(5, D)]]
     assert ((rest - 1).abs() <= half_step(BF16) + 2 * (n + 64) * half_step(FP32)).all()
+
+
+# ---- forward-mode derivatives ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["q", "k", "cos", "grad"])
+def test_rotary_drops_no_tangent(device, which):
+    """The rotation is linear: its tangent is that of the input, rotated, as on the host, or the call is refused."""
+    cos, sin = rope_tables(6, 8, device=device)
+    g = torch.Generator().manual_seed(3)
+    q, k, dq = (torch.randn(1, 2, 6, 8, generator=g).to(device) for _ in range(3))
+    t = torch.randn(1, 2, 6, 8, generator=g).to(device)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(cos, torch.ones_like(cos)) if which == "cos" else forward_ad.make_dual({"q": q, "k": k, "grad": dq}[which], t)
+
+        def call():
+            if which == "grad":
+                x = q.clone().requires_grad_()
+                return torch.autograd.grad(rotary_embedding(x, None, cos, sin), x, dual)[0]
+            y = rotary_embedding(dual if which == "q" else q, dual if which == "k" else k, dual if which == "cos" else cos, sin)
+            return y[which == "k"]
+
+        if device == "cuda":
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        else:
+            assert forward_ad.unpack_dual(call()).tangent is not None
