@@ -285,6 +285,8 @@ void kv_cache_append(at::Tensor cache_k, at::Tensor cache_v, OptTensor k_scale, 
   const Cache c = check_cache(cache_k, cache_v, k_scale, v_scale, max_len, who);
   check_device(k, cache_k, who, "k");
   check_device(v, cache_k, who, "v");
+  check_not_dual(k, who);
+  check_not_dual(v, who);
   const ServingType type = type_of(k, who, false);
   TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.size(0) == c.B &&
                   k.size(1) == c.H && k.size(3) == c.D,
@@ -362,6 +364,7 @@ at::Tensor kv_cache_attend(at::Tensor q, at::Tensor cache_k, at::Tensor cache_v,
   const char* who = "cache_attention";
   const Cache c = check_cache(cache_k, cache_v, k_scale, v_scale, max_len, who);
   check_device(q, cache_k, who, "q");
+  check_not_dual(q, who);
   const ServingType type = type_of(q, who, false);
   TORCH_CHECK(q.dim() == 4 && q.size(0) == c.B && q.size(3) == c.D, who, ": q must be [", c.B, ", Hq, T, ", c.D, "]");
   TORCH_CHECK(c.H > 0 ? q.size(1) % c.H == 0 : q.size(1) == 0, who, ": ", q.size(1),

@@ -39,6 +39,12 @@ def _no_grad(who, *tensors):
         raise RuntimeError(f"{who} has no backward pass: call it under torch.no_grad()")
 
 
+def _no_tangent(who, *tensors):  # the bindings check this where the kernels run
+    _need(
+        all(torch.autograd.forward_ad.unpack_dual(t).tangent is None for t in tensors), f"{who} has no forward-mode derivative"
+    )
+
+
 class KVCache:
     """Keys and values of one layer: ``batch_size`` sequences, ``num_kv_heads`` heads, up to ``max_len`` tokens.
 
@@ -120,6 +126,7 @@ class KVCache:
         if self._k.is_cuda:
             _load_extension(required=True).kv_cache_append(*self._held(), k, v, self.lengths, offset, counts)
             return
+        _no_tangent("KVCache.append", k, v)
         B, H, _, D = self._k.shape
         _need(
             k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and (k.shape[0], k.shape[1], k.shape[3]) == (B, H, D),
@@ -246,7 +253,7 @@ def cache_attention(
     ``draft_tree_mask``). Without a mask query i sees the new slots 0..i. A query that sees nothing gets zeros. The
     values of slots that a query does not see, NaN among them, do not reach it. ``scale`` defaults to 1 / sqrt(D).
     q is of the cache's type; an 8-bit cache takes bf16 and fp16. The result [B, Hq, T, D] is laid out [B, T, Hq, D] in
-    memory. There is no backward pass.
+    memory. There is no backward pass and no forward-mode derivative.
     """
     _no_grad("cache_attention", q)
     if scale is None:
@@ -256,6 +263,7 @@ def cache_attention(
     if cache._k.is_cuda:
         return _load_extension(required=True).kv_cache_attend(q, *cache._held(), cache.lengths, mask, scale)
 
+    _no_tangent("cache_attention", q)
     B, H, _, D = cache._k.shape
     _need(q.dim() == 4 and q.shape[0] == B and q.shape[3] == D, f"cache_attention: q must be [{B}, Hq, T, {D}]")
     Hq, T = q.shape[1:3]

@@ -123,3 +123,16 @@ def test_rotary_drops_no_tangent(device, which):
                 call()
         else:
             assert forward_ad.unpack_dual(call()).tangent is not None
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_cache_drops_no_tangent(device):
+    cache = KVCache(1, 1, 8, 32, dtype=BF16, device=device)
+    x = torch.ones(1, 1, 2, 32, dtype=BF16, device=device)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x.clone())
+        for call in (lambda: cache.append(dual, x), lambda: cache.append(x, dual), lambda: cache_attention(dual, cache)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        cache.append(x, x)
+        cache_attention(x, cache)
