@@ -497,7 +497,7 @@ class LlamaForCausalLM(nn.Module):
             """One token of each distribution [B, V]."""
             return verify_draft(probs[:, None], root.new_zeros(B, 1), numbers(1)).tokens
 
-        root = input_ids.new_zeros(B, 1)
+        root = torch.zeros(B, 1, dtype=torch.int64, device=device)
         logits = self(input_ids, kv_caches=caches, prefill=True, rope=rope)["logits"][:, -1]
         root = draw(self._target_probs(logits, temperature))
         if draft_model is not None:
@@ -566,7 +566,7 @@ class LlamaForCausalLM(nn.Module):
                     s += t[: n + 1]
             last = torch.gather(verdict.tokens, 1, verdict.counts[:, None])
             root = torch.where(torch.tensor(going, device=device)[:, None], last, root)
-        new = torch.tensor([s[:max_new_tokens] for s in said], device=device, dtype=input_ids.dtype)
+        new = torch.tensor([s[:max_new_tokens] for s in said], device=device)
         return torch.cat((input_ids, new), dim=1)
 
 

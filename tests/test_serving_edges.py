@@ -7,6 +7,7 @@ import torch
 from torch.autograd import forward_ad
 
 from accelerate_amd.ops import KVCache, cache_attention, rope_tables, rotary_embedding
+from test_serving_generate import models, prompt
 
 gpu = pytest.mark.gpu
 DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
@@ -136,3 +137,18 @@ def test_the_cache_drops_no_tangent(device):
                 call()
         cache.append(x, x)
         cache_attention(x, cache)
+
+
+# ---- generate -------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_int32_prompt_generates_what_an_int64_one_does(device):
+    target, draft = models(device)
+    ids = prompt(device)
+    calls = [{}, {"cache_dtype": "int8"}, {"draft_model": draft}, {"draft_model": draft, "draft_widths": (2, 1)}]
+    for kwargs in calls + [{"cache_dtype": "int8", "graph_decode": True}]:
+        for n in (1, 4):
+            want = target.generate(ids, max_new_tokens=n, **kwargs)
+            got = target.generate(ids.int(), max_new_tokens=n, **kwargs)
+            assert got.dtype == torch.int64 and torch.equal(got, want)
