@@ -444,7 +444,7 @@ class LlamaForCausalLM(nn.Module):
     def _generate_served(
         self, input_ids, max_new_tokens, graph_decode, cache_dtype, draft_model, draft_widths, temperature, generator
     ):
-        from ..ops.speculative import verify_draft
+        from ..ops.speculative import MAX_NODES, verify_draft
 
         B, S = input_ids.shape
         device, dtype = input_ids.device, self.lm_head.weight.dtype
@@ -468,6 +468,8 @@ class LlamaForCausalLM(nn.Module):
                 raise ValueError(f"draft_widths must be between 1 and the vocabulary's size, got {draft_widths}")
             for width in draft_widths:
                 first, last = levels[-1]
+                if len(parents) + (last - first) * width > MAX_NODES:
+                    raise ValueError(f"draft_widths {draft_widths} make more than {MAX_NODES} nodes")
                 parents += [node for node in range(first, last) for _ in range(width)]
                 levels.append((last, len(parents)))
         nodes = len(parents)

@@ -13,7 +13,7 @@ import torch
 
 from . import _load_extension
 
-_MAX_NODES = 1024
+MAX_NODES = 1024  # of a draft, root included
 
 
 class DraftVerdict(NamedTuple):
@@ -59,7 +59,7 @@ def verify_draft(
 
     need(target_probs.dim() == 3 and target_probs.is_floating_point(), "target_probs must be a [B, T, V] tensor")
     B, T, V = target_probs.shape
-    need(1 <= T <= _MAX_NODES, f"1 to {_MAX_NODES} nodes, got {T}")
+    need(1 <= T <= MAX_NODES, f"1 to {MAX_NODES} nodes, got {T}")
     need(V >= 1, "an empty vocabulary")
     need(
         draft_probs is None or parents is None,

@@ -152,3 +152,14 @@ def test_an_int32_prompt_generates_what_an_int64_one_does(device):
             want = target.generate(ids, max_new_tokens=n, **kwargs)
             got = target.generate(ids.int(), max_new_tokens=n, **kwargs)
             assert got.dtype == torch.int64 and torch.equal(got, want)
+
+
+def test_generate_refuses_trees_beyond_what_is_verified():
+    target, draft = models("cpu")
+    ran = []
+    for m in (target, draft):
+        m.register_forward_hook(lambda *a: ran.append(1))
+    for widths in ((32, 32), (1,) * 1024, (97, 97, 97, 97, 97, 97)):  # 1057, 1025 and some 10^12 nodes
+        with pytest.raises(ValueError, match="1024"):
+            target.generate(prompt("cpu"), max_new_tokens=4, draft_model=draft, draft_widths=widths)
+    assert not ran
