@@ -449,7 +449,7 @@ class LlamaForCausalLM(nn.Module):
         B, S = input_ids.shape
         device, dtype = input_ids.device, self.lm_head.weight.dtype
         table = self.rope_cos.shape[0]
-        if temperature < 0:
+        if not temperature >= 0:  # NaN too
             raise ValueError(f"temperature must not be negative, got {temperature}")
         if max_new_tokens < 1 or S < 1 or B < 1:
             raise ValueError("generation needs a prompt and at least one new token")

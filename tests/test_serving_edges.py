@@ -163,3 +163,9 @@ def test_generate_refuses_trees_beyond_what_is_verified():
         with pytest.raises(ValueError, match="1024"):
             target.generate(prompt("cpu"), max_new_tokens=4, draft_model=draft, draft_widths=widths)
     assert not ran
+
+
+def test_generate_refuses_a_temperature_that_is_no_number():
+    target, _ = models("cpu")
+    with pytest.raises(ValueError, match="temperature"):
+        target.generate(prompt("cpu"), max_new_tokens=2, temperature=math.nan)
