@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) verify_walk_kernel(VerifyArgs a) {
           open = __ballot(parent == cur);
         } else {
           const int x = __builtin_amdgcn_readlane(token, at);
-          left -= pi;
+          left -= pi > 0. ? pi : 0.;  // NaN too
           without[n++] = x;
           open &= ~__ballot(token == x);
         }

@@ -105,7 +105,7 @@ def verify_draft(
                 node, refused, left = i, [], 1.0
                 taken.append(i)
             else:
-                left -= p
+                left -= p if p > 0 else 0.0  # NaN too
                 refused.append(x)
         row = target_probs[b, node].double()
         row = torch.where(row > 0, row, 0.0)

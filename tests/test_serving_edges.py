@@ -6,7 +6,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from accelerate_amd.ops import KVCache, cache_attention, rope_tables, rotary_embedding
+from accelerate_amd.ops import KVCache, cache_attention, rope_tables, rotary_embedding, verify_draft
 from test_serving_generate import models, prompt
 
 gpu = pytest.mark.gpu
@@ -169,3 +169,23 @@ def test_generate_refuses_a_temperature_that_is_no_number():
     target, _ = models("cpu")
     with pytest.raises(ValueError, match="temperature"):
         target.generate(prompt("cpu"), max_new_tokens=2, temperature=math.nan)
+
+
+# ---- verification ---------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("before", [1, 70])
+def test_a_refused_token_without_weight_takes_none_from_its_siblings(device, before):
+    """NaN counts as no weight: the siblings after such a token are tested as if it had not been drafted."""
+    V, T = 200, before + 3
+    target = torch.zeros(2, T, V)
+    target[:, :, :before] = math.nan
+    target[:, :, 100], target[:, :, 101] = 0.25, 0.75
+    tokens = torch.tensor([0, *range(before), 100, 101]).repeat(2, 1)
+    parents = torch.tensor([-1] + [0] * (T - 1))
+    u = torch.full((2, T), 0.9)
+    u[0, -2] = 0.2  # below the 0.25 of token 100; the other sequence goes on to token 101 with 0.9 * 0.75
+    out = verify_draft(target.to(device), tokens.to(device), u.to(device), parents=parents.to(device))
+    assert out.counts.tolist() == [1, 1]
+    assert out.tokens[:, 0].tolist() == [100, 101] and out.path[:, 1].tolist() == [T - 2, T - 1]
