@@ -273,6 +273,8 @@ class LlamaForCausalLM(nn.Module):
                 positions = kv_caches[0].lengths.long()[:, None] + after
             kv_caches = [CacheStep(cache, positions, offset, mask, prefill) for cache in kv_caches]
         else:
+            if positions is not None or mask is not None or offset or prefill or rope is not None:
+                raise ValueError("positions, mask, offset, prefill and rope go with the caches of make_serving_caches")
             past = kv_caches[0]["len"] if kv_caches is not None else 0
             cos = self.rope_cos[past:].to(x.device)
             sin = self.rope_sin[past:].to(x.device)

@@ -171,6 +171,18 @@ def test_generate_refuses_a_temperature_that_is_no_number():
         target.generate(prompt("cpu"), max_new_tokens=2, temperature=math.nan)
 
 
+def test_arguments_of_serving_caches_are_refused_without_them():
+    """They were ignored: positions that are given would seem to be followed."""
+    target, _ = models("cpu")
+    ids = prompt("cpu", B=1)
+    rope, positions = target.serving_rope(ids.device), torch.arange(9)[None] + 5
+    mask = torch.ones(9, 9, dtype=torch.bool).tril()
+    for kwargs in ({"positions": positions}, {"mask": mask}, {"offset": 1}, {"prefill": True}, {"rope": rope}):
+        for caches in (None, target.make_kv_caches(1, 12, ids.device, torch.float32)):
+            with pytest.raises(ValueError, match="make_serving_caches"):
+                target(ids, kv_caches=caches, **kwargs)
+
+
 # ---- verification ---------------------------------------------------------------------------------------------------
 
 
