@@ -302,7 +302,11 @@ class LlamaForCausalLM(nn.Module):
         ]
 
     def serving_rope(self, device):
-        """The rotary tables as the kernel reads them: on the device, and fp32 where the model was cast to bf16."""
+        """The model's rotary tables as the kernel reads them: on the device, and in fp32.
+
+        All paths of a model follow its buffers. A cast to bf16 takes those along, so they hold 8 bits of each cosine
+        then, and widening does not bring the others back. A model that is to keep fp32 tables gets them anew after the
+        cast: ``model.rope_cos, model.rope_sin = rope_tables(...)``."""
         return self.rope_cos.to(device).float(), self.rope_sin.to(device).float()
 
     def make_serving_caches(self, batch_size, max_len, device, dtype, quant=None, lengths=None):

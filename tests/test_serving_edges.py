@@ -6,6 +6,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from accelerate_amd.models import LlamaConfig, LlamaForCausalLM
 from accelerate_amd.ops import KVCache, cache_attention, rope_tables, rotary_embedding, verify_draft
 from test_serving_generate import models, prompt
 
@@ -181,6 +182,21 @@ def test_arguments_of_serving_caches_are_refused_without_them():
         for caches in (None, target.make_kv_caches(1, 12, ids.device, torch.float32)):
             with pytest.raises(ValueError, match="make_serving_caches"):
                 target(ids, kv_caches=caches, **kwargs)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_cast_model_serves_with_the_tables_that_it_is_given(device):
+    config = LlamaConfig.tiny(num_hidden_layers=1, max_position_embeddings=300)
+    model = LlamaForCausalLM(config).to(device=device, dtype=BF16)
+    tables = rope_tables(300, config.hidden_size // config.num_attention_heads, config.rope_theta, device=device)
+    rounded = model.serving_rope(torch.device(device))
+    # the buffers hold what the cast left: half a step of bf16, and angles up to 300 that were rounded four times to 32 bits
+    assert all((a - b).abs().max() <= 2**-9 + 300 * 4 * half_step(FP32) for a, b in zip(rounded, tables))
+    model.rope_cos, model.rope_sin = tables
+    for got, table in zip(model.serving_rope(torch.device(device)), tables):
+        assert got.dtype == FP32 and torch.equal(got, table)
+    ids = prompt(device)
+    assert model.generate(ids, max_new_tokens=3, cache_dtype="int8").shape == (3, 12)
 
 
 # ---- verification ---------------------------------------------------------------------------------------------------
