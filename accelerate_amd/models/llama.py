@@ -440,6 +440,12 @@ class LlamaForCausalLM(nn.Module):
         return torch.cat(tokens, dim=1)
 
 
+    def _served_dtype(self, device):
+        """What the layers give their caches: autocast's type within it, else the weights'."""
+        if torch.is_autocast_enabled(device.type):
+            return torch.get_autocast_dtype(device.type)
+        return self.lm_head.weight.dtype
+
     def _target_probs(self, logits, temperature):
         """The distributions that tokens are drawn from: of the most likely token alone at temperature 0."""
         if temperature == 0.0:
@@ -453,7 +459,7 @@ class LlamaForCausalLM(nn.Module):
         from ..ops.speculative import MAX_NODES, verify_draft
 
         B, S = input_ids.shape
-        device, dtype = input_ids.device, self.lm_head.weight.dtype
+        device = input_ids.device
         table = self.rope_cos.shape[0]
         if not temperature >= 0:  # NaN too
             raise ValueError(f"temperature must not be negative, got {temperature}")
@@ -485,12 +491,12 @@ class LlamaForCausalLM(nn.Module):
         mask = draft_tree_mask(parents)
         depth = mask.sum(-1) - 1
 
-        caches = self.make_serving_caches(B, S + max_new_tokens + nodes, device, dtype, cache_dtype)
+        caches = self.make_serving_caches(B, S + max_new_tokens + nodes, device, self._served_dtype(device), cache_dtype)
         lengths = caches[0].lengths
         draft_caches = []
         if draft_model is not None:  # what stands is the same for both models
             draft_caches = draft_model.make_serving_caches(
-                B, S + max_new_tokens + nodes, device, draft_model.lm_head.weight.dtype, cache_dtype, lengths
+                B, S + max_new_tokens + nodes, device, draft_model._served_dtype(device), cache_dtype, lengths
             )
 
         rope = self.serving_rope(device)

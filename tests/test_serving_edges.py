@@ -199,6 +199,25 @@ def test_a_cast_model_serves_with_the_tables_that_it_is_given(device):
     assert model.generate(ids, max_new_tokens=3, cache_dtype="int8").shape == (3, 12)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_fp32_model_generates_under_autocast(device):
+    """Its caches are of the type that autocast gives the projections."""
+    target, draft = models(device, dtype=FP32)
+    ids = prompt(device)
+    calls = [{"cache_dtype": "int8"}, {"draft_model": draft}, {"draft_model": draft, "draft_widths": (2, 2), "cache_dtype": "fp8"}]
+    for kwargs in calls + [{"temperature": 1.0}, {"cache_dtype": "int8", "graph_decode": True}]:
+        with torch.autocast(device, dtype=BF16):
+            out = target.generate(ids, max_new_tokens=8, **kwargs)
+        assert out.shape == (3, 17) and torch.equal(out[:, :9], ids)
+        if "temperature" in kwargs:
+            continue
+        with torch.no_grad():
+            logits = target(out)["logits"][:, 8:-1].float()
+        best, got = logits.amax(-1), logits.gather(-1, out[:, 9:, None])[..., 0]
+        # as in test_drafts_on_gpu_follow_the_model: the best token within the roundings of both ways through the model
+        assert (best - got <= 0.1 * (best - logits.mean(-1))).all()
+
+
 # ---- verification ---------------------------------------------------------------------------------------------------
 
 
