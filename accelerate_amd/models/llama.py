@@ -386,7 +386,10 @@ class LlamaForCausalLM(nn.Module):
         continuations of each node of depth i, which this model verifies in
         one pass. ``temperature`` above 0 samples (numbers from
         ``generator``); a draft of widths 1 is sampled then too. Neither the
-        draft nor its shape changes the distribution of what comes out."""
+        draft nor its shape changes the distribution of what comes out, but
+        for the rounding of other products: near ties of the greedy choice
+        may fall otherwise. On the GPU these need a bf16 or fp16 model, or
+        autocast around the call."""
         if cache_dtype is not None or draft_model is not None or temperature != 0.0:
             return self._generate_served(
                 input_ids, max_new_tokens, bool(graph_decode), cache_dtype, draft_model, draft_widths, temperature,

@@ -29,8 +29,8 @@
 // and sequences to fill the chip; a second kernel joins the parts.
 //
 // Measured: 32 sequences of 8000 to 16000 int8 tokens, 64 query heads on 8:
-// 151 us, 5.4 TB/s; one of 130001 bf16 tokens: 93 us, 5.7 TB/s (a large copy:
-// 5.1). One of 300: 7.7 us, the latency of a launch and three readings in turn.
+// 151 us, 5.4 TB/s; one of 130001 bf16 tokens: 93 us, 5.7 TB/s (a stream that
+// only reads: 5.9 to 6.2). One of 300: 7.7 us, the latency of a launch and three readings in turn.
 // Of 108 rows (27 drafted tokens, 4 heads a group) over 8 sequences of 2000 to
 // 4000 e4m3 tokens: 36 us, where the bytes would take 11: two waves a SIMD take
 // about 1600 cycles a tile (1130 of vector and 770 of matrix instructions, which

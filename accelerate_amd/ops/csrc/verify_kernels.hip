@@ -18,8 +18,8 @@
 // tokens by about their own width.
 //
 // Bound by latency and then by reading one row (with q two) a sequence: 8 chains
-// of 5 drafts over 128256 tokens take 5.5 us and 5.8 for the two kernels, 2
-// trees of 22 nodes over 50257 about as much (captured, 10.1 a call). The
+// of 5 drafts over 128256 tokens take 5.4 us for each of the two kernels and
+// 10.8 a captured call, 2 trees of 22 nodes over 50257 4.9 each and 9.8. The
 // walk needs one value (two) a node, read by a thread each, and is done by
 // every workgroup for itself, so that a grid over chunks of the vocabulary
 // can sum its row at once, without a launch between; a second kernel finds
