@@ -444,6 +444,9 @@ struct Rows : Shape<T, kKind, kD> {
       for (int e = 2; e < 8; ++e) top = fmaxf(top, p[mt][e]);
       top = max_over_groups(top);
       if constexpr (!S::kScaled) top *= scale;
+      // Not below the product as it is, half a step of which was rounded off:
+      // a probability above 1 would leave fp16's range (from scores of 2^24 on).
+      if constexpr (kLift != 1.f) top = __builtin_fmaf(fabsf(top), 0x1p-23f, top);
       const float m_new = fmaxf(m[mt], top);
       keep[mt] = __builtin_amdgcn_exp2f(m[mt] - m_new);
       grew |= m_new > m[mt];

@@ -76,6 +76,28 @@ def test_a_large_value_of_low_weight_leaves_the_others_their_bits_in_fp16(quant,
     check_weighted(cache_attention(q, cache, scale=0.125), q, cache, 0.125)
 
 
+@gpu
+@pytest.mark.parametrize("quant", [None, "int8", "fp8"])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("n", [40, 1000])
+def test_scores_beyond_whole_numbers_of_32_bits(quant, dtype, n):
+    """Products of 2^24 and more, where 32 bits step by 2 to 32: the largest score has all the weight, and no more."""
+    D, heads = 64, 32
+    g = torch.Generator().manual_seed(4)
+    cache = KVCache(1, 1, n, D, dtype=dtype, quant=quant, device="cuda")
+    size = torch.full((n,), 0.5)
+    size[n // 3], size[-1] = 1.0, 0.75  # scores lie 2^22 apart
+    k = (1500 * size[:, None]).expand(n, D).to(dtype)
+    v = torch.randn(n, D, generator=g).to(dtype)
+    cache.append(k[None, None].cuda(), v[None, None].cuda())
+    cache.lengths.fill_(n - 1)
+    q = (1500 + 200 * torch.arange(heads))[:, None].expand(heads, D).to(dtype)[None, :, None]
+    out = cache_attention(q.cuda(), cache)[0, :, 0].double().cpu()
+    want = cache.read(dtype=FP32)[1][0, 0, n // 3].double().cpu().expand(heads, D)
+    # the token's value times its weight over itself: 16 bits of the weight, a division, and the result's own rounding
+    assert ((out - want).abs() <= (half_step(dtype) + 2**-16 + 4 * half_step(FP32)) * want.abs() + 2.0**-25).all()
+
+
 # ---- attention: infinities ------------------------------------------------------------------------------------------
 
 
